@@ -37,6 +37,7 @@ typedef struct ornith_hip_ctx ornith_hip_ctx;
 typedef struct ornith_hip_tensor ornith_hip_tensor;
 typedef struct ornith_hip_model ornith_hip_model;
 typedef struct ornith_hip_session ornith_hip_session;
+typedef struct ornith_hip_paged ornith_hip_paged;
 
 /* Q8_K activation super-block, byte-identical to oq8k_block
  * (src/ornith_qdot.h:30-34): 292 bytes. */
@@ -235,6 +236,98 @@ int  ornith_hip_session_get_kv(ornith_hip_session *s, int layer, int8_t *Kq,
  * full attention. */
 int  ornith_hip_session_get_attn(ornith_hip_session *s, int row, float *q, float *gate, float *o,
                                  int32_t *pos);
+
+/* ---- paged key/value pool (no reference twin; device buffers) ------------------ */
+
+/* The cache of many requests in the pages of one pool per attention layer, for
+ * a scheduler that runs a batch of them at once. Rows, lists and the workspace
+ * are device memory of the context's device; every call of this section but
+ * _new, _free and _faults only enqueues on `stream` (a hipStream_t of that
+ * device; NULL: its null stream), allocates nothing and may be captured into a
+ * graph. Calls on one pool are ordered by the caller's streams; calls that
+ * overlap need workspaces of their own, and must not append to a page that
+ * another one reads or writes. The lists are read on the device when the call
+ * runs there, so that a replayed graph sees their present contents.
+ *
+ * Types: rows F32 (0), F16 (1) or BF16 (30). */
+#define ORNITH_HIP_KV_F16  1
+#define ORNITH_HIP_KV_Q8   8    /* int8 codes, one f32 scale per position and head: rint(x * 127 / max|x|), max|x| / 127 */
+#define ORNITH_HIP_KV_BF16 30
+
+typedef struct {
+    int32_t nkv, hd;            /* key/value heads; head dim: 64, 128 or 256 */
+    int32_t page_len, n_pages;  /* positions a page: 32, 64, 128 or 256 */
+    uint32_t type;              /* ORNITH_HIP_KV_*; a 16-bit pool takes rows of its own type, a Q8 one any */
+    int32_t rope_dim;           /* rotated dims of a head (pairs i, i + rope_dim / 2); 0: no rotation */
+    float rope_theta;           /* frequencies theta^(-2i / rope_dim); angles are formed in 64 bits */
+    int32_t max_pos;            /* rotation positions are below this (at most 2^24) */
+    const uint8_t *rope_axis;   /* host: axis (0 to 3) of each of the rope_dim / 2 frequencies; NULL: all 0 */
+} ornith_hip_paged_cfg;
+
+/* A ragged batch. Sequence s owns the rows [seq_start[s], seq_start[s + 1]); its
+ * last row is at position kv_len[s] - 1 (kv_len counts the rows of this call),
+ * the others before it, and position p is in page pages[s * max_pages + p /
+ * page_len]. Rows at negative positions are padding, and rows behind
+ * seq_start[n_seq] nobody's. Entries of `pages` that no position needs are not
+ * looked at. */
+typedef struct {
+    const int32_t *seq_start;   /* [n_seq + 1], ascending */
+    const int32_t *kv_len;      /* [n_seq] */
+    const int32_t *pages;       /* [n_seq][max_pages] */
+    int32_t n_seq, n_rows;      /* rows that the row buffers hold */
+    int32_t max_pages;
+    int32_t max_new;            /* no sequence has more rows than this */
+} ornith_hip_paged_batch;
+
+/* Rows of heads: element (row, head, d) at p[row * row_stride + head *
+ * head_stride + d]; pointer and strides (in elements) are multiples of 16 bytes. */
+typedef struct { void *p; int64_t row_stride, head_stride; } ornith_hip_rows;
+
+int  ornith_hip_paged_new(ornith_hip_ctx *ctx, const ornith_hip_paged_cfg *cfg, ornith_hip_paged **out);
+/* Like models and sessions a pool may be freed after its context. The work on
+ * it has to be done, and graphs that use it are not launched any more. */
+void ornith_hip_paged_free(ornith_hip_paged *p);
+/* What the lists of earlier calls had wrong, as bits, and forgets it: 1 a page
+ * outside the pool (its positions are neither written nor seen), 2 a rotation
+ * position outside [0, max_pos) (the row is neither stored nor rotated), 4
+ * seq_start, kv_len, max_new or a prefix out of range (the sequence's rows, or
+ * the row, are left out). Waits for the device. */
+int  ornith_hip_paged_faults(ornith_hip_paged *p, int32_t *faults);
+
+/* Store the batch's rows of keys and values at their positions. Keys are
+ * normed first if k_norm is given (hd weights, x / sqrt(mean(x^2) + eps) * w), then
+ * rotated; queries likewise (nh heads, q_norm), into q_out, which may be q
+ * itself but not overlap it otherwise; q NULL: none. Rotation positions:
+ * rope_pos[axis * rope_stride + row], or NULL: the cache position. */
+int  ornith_hip_paged_append(ornith_hip_paged *p, const ornith_hip_paged_batch *b, int nh, uint32_t type,
+                             const ornith_hip_rows *k, const ornith_hip_rows *v, const ornith_hip_rows *q,
+                             const ornith_hip_rows *q_out, const float *q_norm, const float *k_norm, float eps,
+                             const int32_t *rope_pos, int64_t rope_stride, void *stream);
+/* The keys and values stored at the batch's rows (a whole sequence: kv_len
+ * rows). Padding and nobody's rows are left as they were. */
+int  ornith_hip_paged_read(const ornith_hip_paged *p, const ornith_hip_paged_batch *b, uint32_t type,
+                           const ornith_hip_rows *k, const ornith_hip_rows *v, void *stream);
+
+/* Causal attention of the batch's rows over their sequences' positions, up to
+ * and with their own: out = sum_t softmax_t(scale * q . k_t) v_t, nh query
+ * heads over nkv (nh % nkv == 0, head h reads h / (nh / nkv)). Padding rows get
+ * 0, nobody's are left as they were. out must not overlap q. The workspace
+ * (16-byte aligned, contents undefined before and after) is at least what
+ * ornith_hip_paged_workspace says for the batch's sizes. */
+int  ornith_hip_paged_workspace(const ornith_hip_paged *p, const ornith_hip_paged_batch *b, int nh, int n_group,
+                                uint64_t *bytes);
+int  ornith_hip_paged_attend(const ornith_hip_paged *p, const ornith_hip_paged_batch *b, int nh, uint32_t type,
+                             const ornith_hip_rows *q, const ornith_hip_rows *out, float scale, void *workspace,
+                             uint64_t workspace_bytes, void *stream);
+/* The same for groups of sequences that begin alike: those in [prefix_first[i],
+ * prefix_first[i + 1]) (device, n_group + 1 entries, ascending) have the same
+ * pages for the whole pages within their first prefix_len[i] positions (device,
+ * n_group), which are read once for all rows of the group. Sequences outside
+ * every group are as in ornith_hip_paged_attend. */
+int  ornith_hip_paged_attend_prefix(const ornith_hip_paged *p, const ornith_hip_paged_batch *b, int n_group,
+                                    const int32_t *prefix_first, const int32_t *prefix_len, int nh, uint32_t type,
+                                    const ornith_hip_rows *q, const ornith_hip_rows *out, float scale, void *workspace,
+                                    uint64_t workspace_bytes, void *stream);
 
 /* ---- measurement (no reference twin) -------------------------------------------- */
 

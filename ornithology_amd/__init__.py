@@ -49,6 +49,24 @@ class Arch(C.Structure):
         ("rope_theta", C.c_float), ("eps", C.c_float), ("eos", C.c_int32)]
 
 
+# types of a paged pool (ORNITH_HIP_KV_*)
+KV_F16, KV_Q8, KV_BF16 = 1, 8, 30
+
+
+class PagedCfg(C.Structure):
+    _fields_ = [("nkv", C.c_int32), ("hd", C.c_int32), ("page_len", C.c_int32), ("n_pages", C.c_int32), ("type", C.c_uint32),
+                ("rope_dim", C.c_int32), ("rope_theta", C.c_float), ("max_pos", C.c_int32), ("rope_axis", C.c_void_p)]
+
+
+class _Batch(C.Structure):
+    _fields_ = [("seq_start", C.c_void_p), ("kv_len", C.c_void_p), ("pages", C.c_void_p), ("n_seq", C.c_int32),
+                ("n_rows", C.c_int32), ("max_pages", C.c_int32), ("max_new", C.c_int32)]
+
+
+class _Rows(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
 class GenCfg(C.Structure):
     _fields_ = [(n, C.c_int32) for n in (
         "hidden", "n_layers", "vocab", "full_interval", "nh", "nkv", "hd",
@@ -97,6 +115,17 @@ _SIGS = {
     "ornith_hip_session_get_conv": (C.c_int, [_vp, C.c_int, _fp]),
     "ornith_hip_session_get_kv": (C.c_int, [_vp, C.c_int, _vp, _fp, _vp, _fp]),
     "ornith_hip_session_get_attn": (C.c_int, [_vp, C.c_int, _fp, _fp, _fp, _ip]),
+    "ornith_hip_paged_new": (C.c_int, [_vp, C.POINTER(PagedCfg), C.POINTER(_vp)]),
+    "ornith_hip_paged_free": (None, [_vp]),
+    "ornith_hip_paged_faults": (C.c_int, [_vp, _ip]),
+    "ornith_hip_paged_append": (C.c_int, [_vp, C.POINTER(_Batch), C.c_int, C.c_uint32, C.POINTER(_Rows), C.POINTER(_Rows),
+                                          C.POINTER(_Rows), C.POINTER(_Rows), _vp, _vp, C.c_float, _vp, C.c_int64, _vp]),
+    "ornith_hip_paged_read": (C.c_int, [_vp, C.POINTER(_Batch), C.c_uint32, C.POINTER(_Rows), C.POINTER(_Rows), _vp]),
+    "ornith_hip_paged_workspace": (C.c_int, [_vp, C.POINTER(_Batch), C.c_int, C.c_int, C.POINTER(C.c_uint64)]),
+    "ornith_hip_paged_attend": (C.c_int, [_vp, C.POINTER(_Batch), C.c_int, C.c_uint32, C.POINTER(_Rows), C.POINTER(_Rows),
+                                          C.c_float, _vp, C.c_uint64, _vp]),
+    "ornith_hip_paged_attend_prefix": (C.c_int, [_vp, C.POINTER(_Batch), C.c_int, _vp, _vp, C.c_int, C.c_uint32,
+                                                 C.POINTER(_Rows), C.POINTER(_Rows), C.c_float, _vp, C.c_uint64, _vp]),
     "ornith_hip_session_time_decode": (C.c_int, [_vp, C.c_int, _fp]),
     "ornith_hip_time_matvec": (C.c_int, [_vp, _vp, C.c_int, _fp]),
     "ornith_hip_time_matvec_set": (C.c_int, [_vp, C.POINTER(_vp), C.c_int, C.c_int, _fp]),
@@ -148,7 +177,7 @@ class Context:
         L = lib()
         h = _vp()
         _check(L.ornith_hip_init(device, C.byref(h)), "ornith_hip_init")
-        self.h = h
+        self.h, self.device = h, device
 
     def sync(self) -> None:
         _check(lib().ornith_hip_sync(self.h), "ornith_hip_sync")
@@ -216,6 +245,12 @@ class Context:
         h = _vp()
         _check(lib().ornith_hip_model_load(self.h, str(path).encode(), C.byref(h)), "ornith_hip_model_load")
         return Model(self, h)
+
+    def paged_kv(self, n_pages: int, nkv: int, hd: int, *, page_len: int = 64, type: int = KV_Q8, rope_dim: int = 0,
+                 rope_theta: float = 1e7, max_pos: int = 1 << 20, rope_axis=None) -> "PagedKV":
+        """A paged key/value pool (ornith_hip_paged_new); rope_axis: the axis of
+        each of the rope_dim / 2 frequencies."""
+        return PagedKV(self, n_pages, nkv, hd, page_len, type, rope_dim, rope_theta, max_pos, rope_axis)
 
     def synth(self, **cfg) -> "Model":
         c = GenCfg(**cfg)
@@ -480,6 +515,196 @@ class Session:
         if self.h:
             lib().ornith_hip_session_free(self.h)
             self.h = None
+
+
+# ---- paged key/value pool: device buffers, as torch tensors -----------------------
+
+def _torch():
+    """torch, for the calls on device tensors. It brings a HIP runtime of its own,
+    which the library shares if torch is imported before its first use."""
+    import torch
+    return torch
+
+
+_row_types = {}
+
+
+def _row_type(dtype) -> int:
+    if not _row_types:
+        t = _torch()
+        _row_types.update({t.float32: F32, t.float16: F16, t.bfloat16: BF16})
+    if dtype not in _row_types:
+        raise ValueError(f"rows of {dtype}: float32, float16 or bfloat16")
+    return _row_types[dtype]
+
+
+class PagedBatch:
+    """A ragged batch over a pool's pages (ornith_hip_paged_batch): int32 device
+    tensors seq_start [n_seq + 1], kv_len [n_seq] and pages [n_seq, max_pages],
+    whose contents may change between calls; n_rows and max_new are host numbers
+    (default: max_new = n_rows)."""
+
+    def __init__(self, seq_start, kv_len, pages, *, n_rows: int, max_new: int | None = None):
+        t = _torch()
+        n = kv_len.numel()
+        for name, x, shape in (("seq_start", seq_start, (n + 1,)), ("kv_len", kv_len, (n,)), ("pages", pages, (n, pages.shape[-1]))):
+            if x.dtype != t.int32 or tuple(x.shape) != shape or not x.is_contiguous() or x.device.type != "cuda":
+                raise ValueError(f"PagedBatch: {name} is {x.dtype} {tuple(x.shape)} on {x.device}, not contiguous int32 {shape} on the GPU")
+            if x.device != kv_len.device:
+                raise ValueError("PagedBatch: lists on different devices")
+        self.seq_start, self.kv_len, self.pages, self.n_rows = seq_start, kv_len, pages, int(n_rows)
+        self.device = kv_len.device
+        self.c = _Batch(seq_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr(), n, self.n_rows, pages.shape[1],
+                        self.n_rows if max_new is None else int(max_new))
+
+
+class PagedKV:
+    """A paged key/value pool and the operators on it (ornith_hip_paged_*), on
+    torch tensors of the pool's device and on torch's current stream. Rows are
+    [n_rows, heads, hd], each row and head at a multiple of 16 bytes."""
+
+    FAULTS = {1: "a page outside the pool", 2: "a rotation position outside [0, max_pos)",
+              4: "seq_start, kv_len, max_new or a prefix out of range"}
+
+    def __init__(self, ctx: Context, n_pages, nkv, hd, page_len, type, rope_dim, rope_theta, max_pos, rope_axis):
+        t, self.h = _torch(), None
+        axis = None
+        if rope_axis is not None:
+            axis = np.ascontiguousarray(rope_axis, np.uint8)
+            if axis.size != rope_dim // 2 or not np.array_equal(axis, rope_axis):
+                raise ValueError(f"rope_axis: {axis.size} axes for {rope_dim // 2} frequencies, or not 0 to 255")
+        cfg = PagedCfg(nkv, hd, page_len, n_pages, type, rope_dim, rope_theta, max_pos, axis.ctypes.data if axis is not None else None)
+        h = _vp()
+        _check(lib().ornith_hip_paged_new(ctx.h, C.byref(cfg), C.byref(h)), "ornith_hip_paged_new")
+        self.ctx, self.h = ctx, h
+        self.n_pages, self.nkv, self.hd, self.page_len, self.type = n_pages, nkv, hd, page_len, type
+        self.axes = 1 + (int(axis.max()) if axis is not None and axis.size else 0)
+        self.device = t.device("cuda", ctx.device)
+        probe = t.empty(1, device=self.device)
+        if lib().hipPointerGetAttributes(C.create_string_buffer(256), C.c_void_p(probe.data_ptr())) != 0:
+            self.free()
+            raise RuntimeError("torch uses another copy of the HIP runtime than libornith_hip.so: import torch before the "
+                               "first use of ornithology_amd")
+
+    def _rows(self, name, x, heads, n_rows, dtype):
+        if x.dtype != dtype or x.dim() != 3 or x.shape[1] != heads or x.shape[2] != self.hd or x.shape[0] < n_rows:
+            raise ValueError(f"{name} is {x.dtype} {tuple(x.shape)}, not {dtype} [{n_rows}, {heads}, {self.hd}]")
+        if x.device != self.device or x.stride(2) != 1:
+            raise ValueError(f"{name}: on {x.device} (the pool on {self.device}) with strides {x.stride()}; heads are contiguous")
+        if x.requires_grad and _torch().is_grad_enabled():
+            raise ValueError(f"{name} requires a gradient: these operators have no backward pass")
+        return _Rows(x.data_ptr(), x.stride(0) if x.shape[0] > 1 else 0, x.stride(1) if heads > 1 else 0)
+
+    def _begin(self, batch):
+        if self.h is None:
+            raise ValueError("the pool is freed")
+        if batch.device != self.device:
+            raise ValueError(f"the batch is on {batch.device}, the pool on {self.device}")
+        return C.c_void_p(_torch().cuda.current_stream(self.device).cuda_stream)
+
+    def _vector(self, name, x):
+        if x is None:
+            return None
+        t = _torch()
+        if x.dtype != t.float32 or x.numel() != self.hd or not x.is_contiguous() or x.device != self.device:
+            raise ValueError(f"{name}: {self.hd} contiguous float32 weights on {self.device}")
+        return C.c_void_p(x.data_ptr())
+
+    def append(self, batch: PagedBatch, k, v, *, q=None, q_out=None, q_norm=None, k_norm=None, eps: float = 1e-6, rope_pos=None):
+        """Store the batch's rows of keys (normed, rotated) and values, and
+        return q normed and rotated (in q_out, a new tensor by default).
+        rope_pos: int32 [axes, n_rows], default: the cache positions."""
+        t, st = _torch(), self._begin(batch)
+        n = batch.n_rows
+        nh, rq, ro = 0, None, None
+        rk, rv = (self._rows(w, x, self.nkv, n, k.dtype) for w, x in (("k", k), ("v", v)))
+        if q is not None:
+            nh = q.shape[1]
+            if q_out is None:
+                q_out = t.empty((q.shape[0], nh, self.hd), dtype=q.dtype, device=q.device)
+            rq, ro = (C.byref(self._rows(w, x, nh, n, k.dtype)) for w, x in (("q", q), ("q_out", q_out)))
+        stride = 0
+        if rope_pos is not None:
+            if rope_pos.dtype != t.int32 or rope_pos.dim() != 2 or rope_pos.shape[0] < self.axes or rope_pos.shape[1] < n or \
+                    (n > 1 and rope_pos.stride(1) != 1) or rope_pos.device != self.device:
+                raise ValueError(f"rope_pos is {rope_pos.dtype} {tuple(rope_pos.shape)}, not int32 [{self.axes}, {n}] on {self.device}")
+            stride = rope_pos.stride(0)
+        _check(lib().ornith_hip_paged_append(
+            self.h, C.byref(batch.c), nh, _row_type(k.dtype), C.byref(rk), C.byref(rv), rq, ro, self._vector("q_norm", q_norm),
+            self._vector("k_norm", k_norm), eps, None if rope_pos is None else C.c_void_p(rope_pos.data_ptr()), stride, st),
+            "ornith_hip_paged_append")
+        return q_out
+
+    def read(self, batch: PagedBatch, dtype, k=None, v=None):
+        """(k, v): what is stored at the batch's rows, as values of `dtype`."""
+        t, st = _torch(), self._begin(batch)
+        k, v = (t.empty((batch.n_rows, self.nkv, self.hd), dtype=dtype, device=self.device) if x is None else x for x in (k, v))
+        rk, rv = (self._rows(w, x, self.nkv, batch.n_rows, dtype) for w, x in (("k", k), ("v", v)))
+        _check(lib().ornith_hip_paged_read(self.h, C.byref(batch.c), _row_type(dtype), C.byref(rk), C.byref(rv), st),
+               "ornith_hip_paged_read")
+        return k, v
+
+    def workspace(self, batch: PagedBatch, nh: int, n_group: int = 0) -> int:
+        """Bytes of workspace that attend (attend_prefix) needs for the batch's sizes."""
+        n = C.c_uint64(0)
+        _check(lib().ornith_hip_paged_workspace(self.h, C.byref(batch.c), nh, n_group, C.byref(n)), "ornith_hip_paged_workspace")
+        return n.value
+
+    def attend(self, batch: PagedBatch, q, *, scale: float | None = None, out=None, workspace=None):
+        """Causal attention of the batch's rows (ornith_hip_paged_attend); scale:
+        hd ** -0.5 by default. The workspace (a byte tensor) is made per call
+        unless given."""
+        return self._attend(batch, q, scale, out, workspace, None, None)
+
+    def attend_prefix(self, batch: PagedBatch, q, prefix_first, prefix_len, *, scale: float | None = None, out=None, workspace=None):
+        """attend for groups of sequences whose first pages are the same
+        (ornith_hip_paged_attend_prefix): int32 prefix_first [n_group + 1] and
+        prefix_len [n_group]."""
+        t = _torch()
+        for name, x, n in (("prefix_first", prefix_first, prefix_len.numel() + 1), ("prefix_len", prefix_len, prefix_len.numel())):
+            if x.dtype != t.int32 or x.numel() != n or not x.is_contiguous() or x.device != batch.device:
+                raise ValueError(f"{name}: {n} contiguous int32 on {batch.device}")
+        return self._attend(batch, q, scale, out, workspace, prefix_first, prefix_len)
+
+    def _attend(self, batch, q, scale, out, workspace, first, length):
+        t, st = _torch(), self._begin(batch)
+        nh = q.shape[1] if q.dim() == 3 else 0
+        rq = self._rows("q", q, nh, batch.n_rows, q.dtype)
+        if out is None:
+            out = t.empty((q.shape[0], nh, self.hd), dtype=q.dtype, device=q.device)
+        ro = self._rows("out", out, nh, batch.n_rows, q.dtype)
+        n_group = 0 if first is None else length.numel()
+        if workspace is None:
+            need = self.workspace(batch, nh, n_group)
+            workspace = t.empty(need, dtype=t.uint8, device=self.device) if need else None
+        size = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        args = (nh, _row_type(q.dtype), C.byref(rq), C.byref(ro), self.hd ** -0.5 if scale is None else scale,
+                C.c_void_p(workspace.data_ptr()) if size else None, size, st)
+        if first is None:
+            _check(lib().ornith_hip_paged_attend(self.h, C.byref(batch.c), *args), "ornith_hip_paged_attend")
+        else:
+            _check(lib().ornith_hip_paged_attend_prefix(self.h, C.byref(batch.c), n_group, C.c_void_p(first.data_ptr()),
+                                                        C.c_void_p(length.data_ptr()), *args), "ornith_hip_paged_attend_prefix")
+        return out
+
+    def check(self) -> None:
+        """Raise if an earlier call on the pool met lists that are out of range
+        (ornith_hip_paged_faults); waits for the device."""
+        f = C.c_int32(0)
+        _check(lib().ornith_hip_paged_faults(self.h, C.byref(f)), "ornith_hip_paged_faults")
+        if f.value:
+            raise HipError(2, "PagedKV", "; ".join(w for b, w in self.FAULTS.items() if f.value & b))
+
+    def free(self):
+        if self.h:
+            lib().ornith_hip_paged_free(self.h)
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
 
 
 def row_bytes(t: int, n: int) -> int:

@@ -1,0 +1,52 @@
+// oh_paged_dev.h - device helpers of the paged pool's kernels.
+#pragma once
+#include "oh_common.h"
+#include "oh_paged.h"
+
+typedef __bf16 pg_b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 pg_h8 __attribute__((ext_vector_type(8)));
+typedef float pg_f4 __attribute__((ext_vector_type(4)));
+typedef float pg_f16 __attribute__((ext_vector_type(16)));
+
+template <int T> struct pg_elem;                       // storage type of a row or pool element
+template <> struct pg_elem<OH_PT_F32> { typedef float t; };
+template <> struct pg_elem<OH_PT_F16> { typedef _Float16 t; };
+template <> struct pg_elem<OH_PT_BF16> { typedef __bf16 t; };
+template <> struct pg_elem<OH_PT_Q8> { typedef int8_t t; };
+
+OH_DEV void pg_report(const oh_pool &p, int bit) { atomicOr(p.fault, bit); }
+
+// element offsets in a (page, head) block's key and value parts of position
+// `slot` of the page (16-bit and 8-bit pools: units of 8 and 16 elements)
+template <int CT>
+OH_DEV uint32_t pg_k_at(int hd, int slot, int d) {
+    constexpr int U = CT == OH_PT_Q8 ? 16 : 8;
+    return (uint32_t)((slot >> 5) * 32 * hd + ((d / U) * 32 + (slot & 31)) * U + d % U);
+}
+OH_DEV uint32_t pg_v_at(int hd, int slot, int d) {
+    const int s = slot & 31;
+    return (uint32_t)((slot >> 5) * 32 * hd + (((s >> 2) & 3) * hd + d) * 8 + 4 * (s >> 4) + (s & 3));
+}
+OH_DEV uint8_t *pg_block(const oh_pool &p, int page, int head) {
+    return p.mem + ((size_t)page * p.nkv + head) * p.block;
+}
+
+// the sequence that row r belongs to, -1 (and reported) if `start` is no ascending list
+OH_DEV int pg_seq_of(const oh_pool &p, const oh_pbatch &b, int r) {
+    int lo = 0, hi = b.n_seq;                          // the last s with start[s] <= r
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (b.start[mid] <= r) lo = mid; else hi = mid;
+    }
+    const int s0 = b.start[lo], s1 = b.start[lo + 1];
+    if (r < s0 || r >= s1) {
+        // rows behind the last sequence are nobody's; any other such row is a mistake
+        if (r < b.start[b.n_seq]) pg_report(p, OH_PF_BATCH);
+        return -1;
+    }
+    return lo;
+}
+
+// log2 of e
+constexpr float kLog2e = 1.44269504088896340736f;
+OH_DEV float pg_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
