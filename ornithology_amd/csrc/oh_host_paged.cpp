@@ -74,24 +74,34 @@ int row_type(const char *who, const ornith_hip_paged *p, uint32_t type) {
     return ORNITH_HIP_OK;
 }
 
-// Parts of the key axis: enough blocks to fill the card several times over, so
-// that sequences of different lengths even out, and no more than the longest
-// list of pages can need.
-constexpr int kParts = 64, kBlocks = 2048;
-void plan(const ornith_hip_paged *p, const oh_pbatch &b, int nh, oh_pattn *a) {
-    const int G = nh / p->pool.nkv;
-    const int64_t most = (int64_t)b.max_pages << p->pool.page_sh;
-    const int64_t blocks = std::max<int64_t>(1, (int64_t)b.n_seq * p->pool.nkv * (((int64_t)b.max_new * G + 15) / 16));
-    const int64_t n = std::min<int64_t>(kParts, std::min((most + 127) / 128, kBlocks / blocks));
+// Which kernels take the batch, and in how many parts of the key axis: enough
+// blocks to fill the card a few times over, so that sequences of different
+// lengths even out, and no more parts than the longest list of pages can need.
+// A sequence's rows times the heads of a group decide: up to kFewRows they go to
+// the kernel for few rows; where all sequences have more, or could, to the one
+// for many.
+constexpr int kFewRows = 32, kManyRows = 128;
+int parts_of(int64_t most, int64_t blocks, int64_t want, int limit) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>(limit, std::min((most + 127) / 128, want / std::max<int64_t>(1, blocks))));
+}
+void plan(const ornith_hip_paged *p, const oh_pbatch &b, int nh, int n_group, oh_pattn *a) {
+    const int nkv = p->pool.nkv, G = nh / nkv;
+    const int64_t most = (int64_t)b.max_pages << p->pool.page_sh, widest = (int64_t)b.max_new * G, all = (int64_t)b.n_rows * G;
     a->G = G;
     a->nh = nh;
-    a->parts = (int)std::max<int64_t>(1, n);
-    a->gparts = 0;
+    a->n_group = n_group;
+    a->few = widest <= kFewRows || (b.n_seq > 1 && b.n_rows < (int64_t)b.n_seq * b.max_new) ? kFewRows : 0;
+    a->many = widest <= kFewRows ? -1 : a->few;
+    a->gmany = all > kFewRows;
+    a->parts = a->few ? parts_of(most, (int64_t)b.n_seq * nkv, 2048, 64) : 1;
+    a->mparts = a->many >= 0 ? parts_of(most, (all / kManyRows + 1) * nkv, 768, 32) : 1;
+    a->gparts = !n_group ? 0 : a->gmany ? parts_of(most, (all / kManyRows + n_group) * nkv, 512, 64) : parts_of(most, n_group * nkv, 512, 64);
+    a->sparts = std::max(a->parts, a->mparts);
 }
-uint64_t work_bytes(const oh_pattn &a) {
-    if (a.parts == 1 && !a.n_group) return 0;
-    return (uint64_t)a.b.n_rows * a.nh * (a.parts + a.gparts) * ((uint64_t)a.pool.hd * 4 + 8);
+uint64_t work_parts(const oh_pattn &a) {
+    return a.sparts == 1 && !a.n_group ? 0 : (uint64_t)a.b.n_rows * a.nh * (a.sparts + a.gparts);
 }
+uint64_t work_bytes(const oh_pattn &a) { return work_parts(a) * ((uint64_t)a.pool.hd * 4 + 8); }
 
 int heads(const char *who, const ornith_hip_paged *p, int nh) {
     if (nh < 1 || nh % p->pool.nkv) {
@@ -119,19 +129,24 @@ int attend(const char *who, const ornith_hip_paged *p, const ornith_hip_paged_ba
     CHK(rows_of(who, "q", q, type, &a.q));
     CHK(rows_of(who, "out", out, type, &a.out));
     a.pool = p->pool;
-    a.scale = scale * 1.44269504088896340736f;
     a.type = (int)type;
-    plan(p, a.b, nh, &a);
+    a.scale = fabsf(scale) * 1.44269504088896340736f;
+    a.sign = scale < 0.0f ? -1.0f : 1.0f;
+    a.gfirst = first; a.glen = shared;
+    plan(p, a.b, nh, n_group, &a);
     const uint64_t need = work_bytes(a);
     if (need > ws_bytes || (need && (!ws || (uintptr_t)ws % 16))) {
         seterr("%s: a 16-byte aligned workspace of %llu bytes is needed, %llu given", who, (unsigned long long)need, (unsigned long long)ws_bytes);
         return ORNITH_HIP_ERR_FORMAT;
     }
     a.po = (float *)ws;
-    a.pml = (float2 *)(a.po + (uint64_t)a.b.n_rows * nh * (a.parts + a.gparts) * a.pool.hd);
+    a.pml = (float2 *)(a.po + work_parts(a) * a.pool.hd);
     OnDevice dev(p->ctx->device);
     HCHK(dev.e);
-    HCHK(oh_launch_paged_attn(&a, (hipStream_t)stream));
+    const hipStream_t st = (hipStream_t)stream;
+    if (a.many >= 0 || (n_group && a.gmany)) HCHK(oh_launch_pattn_many(&a, st));
+    if (a.few || (n_group && !a.gmany)) HCHK(oh_launch_pattn_few(&a, st));
+    if (need) HCHK(oh_launch_pattn_join(&a, st));
     return ORNITH_HIP_OK;
 }
 
@@ -294,11 +309,11 @@ extern "C" int ornith_hip_paged_workspace(const ornith_hip_paged *p, const ornit
     *bytes = 0;
     CHK(batch_of("paged_workspace", p, b, &a.b));
     CHK(heads("paged_workspace", p, nh));
+    if (n_group < 0) { seterr("paged_workspace: %d groups", n_group); return ORNITH_HIP_ERR_FORMAT; }
     if (nothing(a.b)) return ORNITH_HIP_OK;
     CHK(placed("paged_workspace", b));
     a.pool = p->pool;
-    plan(p, a.b, nh, &a);
-    (void)n_group;
+    plan(p, a.b, nh, n_group, &a);
     *bytes = work_bytes(a);
     return ORNITH_HIP_OK;
 }

@@ -107,6 +107,10 @@ paged_append(oh_pappend a) {
 #pragma unroll
         for (int e = 0; e < E; e++) am = fmaxf(am, fabsf(y[e]));
         am = wave_max_f32(am);
+        bool nan = false;                              // a NaN is in no code: it goes into the scale
+#pragma unroll
+        for (int e = 0; e < E; e++) nan |= y[e] != y[e];
+        if (__any(nan)) am = NAN;
         const float iv = am > 0.0f ? 127.0f / am : 0.0f;
         if (lane == 0) *(float *)(blk + (isv ? a.pool.vs_off : a.pool.ks_off) + 4 * slot) = am / 127.0f;
 #pragma unroll

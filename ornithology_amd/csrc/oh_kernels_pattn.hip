@@ -1,6 +1,7 @@
 // oh_kernels_pattn.hip - attention of a ragged batch over a paged pool, and the
 // joining of partial results.
 #include "oh_pattn_dev.h"
+#include <algorithm>
 
 namespace {
 
@@ -10,7 +11,7 @@ namespace {
 // (lane n = lane & 15 holds row n's scores of positions 4g..4g+3 and
 // 16+4g..+3, g = lane >> 4), the probabilities, and O^T += V^T P^T with the
 // probabilities where they are: the pool's value order matches.
-template <int RT, int CT, int HD>
+template <int RT, int CT, int HD, bool PREFIX>
 __global__ void __launch_bounds__(256)
 pattn_few(oh_pattn a, int tiles_of_rows) {
     typedef typename pg_elem<RT>::t row_t;
@@ -21,25 +22,21 @@ pattn_few(oh_pattn a, int tiles_of_rows) {
     __shared__ float red[4][16][68];
     __shared__ float sm[4][16], sl[4][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    const int s = (int)blockIdx.x / tiles_of_rows, rt = (int)blockIdx.x % tiles_of_rows, kvh = blockIdx.y, c = blockIdx.z;
-    int row0, rows, len;
-    if (!pg_seq(a, s, &row0, &rows, &len)) return;
-    const int G = a.G, F = rows * G;
-    if (rt * 16 >= F) return;
-    int lo = 0;
-    const int grp = pg_group_of(a, s);
-    if (grp >= 0) lo = pg_shared(a, grp);
-    const int parts = pg_parts(len - lo, a.parts);
+    const int unit = (int)blockIdx.x / tiles_of_rows, rt = (int)blockIdx.x % tiles_of_rows, kvh = blockIdx.y, c = blockIdx.z;
+    pg_unit u;
+    if (!pg_unit_at<PREFIX>(a, unit, &u)) return;
+    const int G = a.G, F = u.n * G;
+    if (rt * 16 >= F || (!PREFIX && F > a.few) || (PREFIX && !u.hi)) return;
+    const int parts = pg_parts(u.hi - u.lo, PREFIX ? a.gparts : a.parts);
     if (c >= parts) return;
-    const int64_t all = a.gparts + a.parts;
-    const bool direct = parts == 1 && lo == 0;
-    // this part's tiles (of the page list's 32-position tiles)
-    const int T0 = lo >> 5, T = len > lo ? ((len + 31) >> 5) - T0 : 0;
-    const int t0 = T0 + (int)((int64_t)T * c / parts), t1 = T0 + (int)((int64_t)T * (c + 1) / parts);
+    const int64_t all = a.gparts + a.sparts, pc = PREFIX ? c : a.gparts + c;
+    const bool direct = !PREFIX && parts == 1 && u.lo == 0;
+    int t0, t1;
+    pg_part(u, c, parts, &t0, &t1);
     // this lane's row
-    const int f = rt * 16 + n, tok = row0 + f / G, head = kvh * G + f % G;
+    const int f = rt * 16 + n, tok = u.row + f / G, head = kvh * G + f % G;
     const bool valid = f < F;
-    const int lim = valid ? pg_lim(a, len, row0 + rows, tok) : 0;
+    const int lim = valid ? pg_unit_lim<PREFIX>(a, u, tok) : 0;
     opv qf[NQ][NS];
 #pragma unroll
     for (int i = 0; i < NS; i++) {
@@ -50,7 +47,7 @@ pattn_few(oh_pattn a, int tiles_of_rows) {
         if (valid) {
             const row_t *src = (const row_t *)a.q.p + tok * a.q.rs + head * a.q.hs + d;
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = (float)src[j];
+            for (int j = 0; j < 8; j++) x[j] = (float)src[j] * a.sign;
         }
         opv t[NQ];
         pg_split<NQ>(x, t);
@@ -61,10 +58,9 @@ pattn_few(oh_pattn a, int tiles_of_rows) {
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = (pg_f4){0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
-    const int32_t *pages = a.b.table + (size_t)s * a.b.max_pages;
     const int page_mask = (1 << a.pool.page_sh) - 1;
     for (int t = t0 + wave; t < t1; t += 4) {
-        const int tb = 32 * t, page0 = pages[tb >> a.pool.page_sh];
+        const int tb = 32 * t, page0 = u.pages[tb >> a.pool.page_sh];
         const bool bad = page0 < 0 || page0 >= a.pool.n_pages;   // its positions are seen by no row
         if (bad && lane == 0) pg_report(a.pool, OH_PF_PAGE);
         const uint8_t *blk = pg_block(a.pool, bad ? 0 : page0, kvh);
@@ -74,36 +70,36 @@ pattn_few(oh_pattn a, int tiles_of_rows) {
         const uint8_t *kp = blk + tile, *vp = blk + a.pool.v_off + tile;
         pg_f4 sc[2];
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            sc[u] = (pg_f4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int h = 0; h < 2; h++) {
+            sc[h] = (pg_f4){0.0f, 0.0f, 0.0f, 0.0f};
             if (Q8) {
 #pragma unroll
                 for (int i = 0; i < NS / 2; i++) {
-                    const uint4 w = *(const uint4 *)(kp + ((4 * i + g) * 32 + 16 * u + n) * 16);
+                    const uint4 w = *(const uint4 *)(kp + ((4 * i + g) * 32 + 16 * h + n) * 16);
                     const pg_b8 k0 = pg_codes(w.x, w.y), k1 = pg_codes(w.z, w.w);
 #pragma unroll
                     for (int k = NQ - 1; k >= 0; k--) {          // the small terms first
-                        sc[u] = pg_mma16(__builtin_bit_cast(opv, k0), qf[k][2 * i], sc[u]);
-                        sc[u] = pg_mma16(__builtin_bit_cast(opv, k1), qf[k][2 * i + 1], sc[u]);
+                        sc[h] = pg_mma16(__builtin_bit_cast(opv, k0), qf[k][2 * i], sc[h]);
+                        sc[h] = pg_mma16(__builtin_bit_cast(opv, k1), qf[k][2 * i + 1], sc[h]);
                     }
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < NS; i++)
-                    sc[u] = pg_mma16(*(const opv *)(kp + ((4 * i + g) * 32 + 16 * u + n) * 16), qf[0][i], sc[u]);
+                    sc[h] = pg_mma16(*(const opv *)(kp + ((4 * i + g) * 32 + 16 * h + n) * 16), qf[0][i], sc[h]);
             }
         }
         float p[8];
         float mx = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
+        for (int h = 0; h < 2; h++) {
             pg_f4 ks = {1.0f, 1.0f, 1.0f, 1.0f};
-            if (Q8) ks = *(const pg_f4 *)(blk + a.pool.ks_off + 4 * (slot + 16 * u + 4 * g));
+            if (Q8) ks = *(const pg_f4 *)(blk + a.pool.ks_off + 4 * (slot + 16 * h + 4 * g));
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float x = Q8 ? sc[u][i] * ks[i] * a.scale : sc[u][i] * a.scale;
-                p[4 * u + i] = 16 * u + 4 * g + i < vis ? x : -INFINITY;
-                mx = fmaxf(mx, p[4 * u + i]);
+                const float x = Q8 ? sc[h][i] * ks[i] * a.scale : sc[h][i] * a.scale;
+                p[4 * h + i] = 16 * h + 4 * g + i < vis ? x : -INFINITY;
+                mx = fmaxf(mx, p[4 * h + i]);
             }
         }
         mx = fmaxf(mx, __shfl_xor(mx, 16));
@@ -114,15 +110,15 @@ pattn_few(oh_pattn a, int tiles_of_rows) {
         m = mn;
         l *= alpha;
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
+        for (int h = 0; h < 2; h++) {
             pg_f4 vs = {1.0f, 1.0f, 1.0f, 1.0f};
-            if (Q8) vs = *(const pg_f4 *)(blk + a.pool.vs_off + 4 * (slot + 16 * u + 4 * g));
+            if (Q8) vs = *(const pg_f4 *)(blk + a.pool.vs_off + 4 * (slot + 16 * h + 4 * g));
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const bool see = 16 * u + 4 * g + i < vis;
-                const float e = see ? pg_exp2(p[4 * u + i] - ref) : 0.0f;
+                const bool see = 16 * h + 4 * g + i < vis;
+                const float e = see ? pg_exp2(p[4 * h + i] - ref) : 0.0f;
                 l += e;
-                p[4 * u + i] = Q8 ? (see ? e * vs[i] : 0.0f) : e;
+                p[4 * h + i] = Q8 ? (see ? e * vs[i] : 0.0f) : e;
             }
         }
         opv pf[NP];
@@ -187,11 +183,11 @@ pattn_few(oh_pattn a, int tiles_of_rows) {
 #pragma unroll
     for (int w = 0; w < 4; w++) L += sm[w][n] == -INFINITY ? 0.0f : sl[w][n] * pg_exp2(sm[w][n] - M);
     const float mine = m == -INFINITY ? 0.0f : pg_exp2(m - M);
-    const int64_t part = ((int64_t)tok * a.nh + head) * all + a.gparts + c;
+    const int64_t part = ((int64_t)tok * a.nh + head) * all + pc;
     if (!direct && wave == 0 && g == 0 && valid) a.pml[part] = make_float2(M, L);
     // thread x writes row x >> 4, dims 4 (x & 15) .. + 3 of the 64
     const int wr = threadIdx.x >> 4, wd = 4 * (threadIdx.x & 15), wf = rt * 16 + wr;
-    const int wtok = row0 + wf / G, whead = kvh * G + wf % G;
+    const int wtok = u.row + wf / G, whead = kvh * G + wf % G;
     float Lw = 0.0f, Mw = -INFINITY;
 #pragma unroll
     for (int w = 0; w < 4; w++) Mw = fmaxf(Mw, sm[w][wr]);
@@ -220,7 +216,7 @@ pattn_few(oh_pattn a, int tiles_of_rows) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) to[i] = (row_t)y[i];
             } else {
-                *(pg_f4 *)(a.po + (((int64_t)wtok * a.nh + whead) * all + a.gparts + c) * HD + 64 * q + wd) = (pg_f4){y[0], y[1], y[2], y[3]};
+                *(pg_f4 *)(a.po + (((int64_t)wtok * a.nh + whead) * all + pc) * HD + 64 * q + wd) = (pg_f4){y[0], y[1], y[2], y[3]};
             }
         }
     }
@@ -239,10 +235,10 @@ pattn_join(oh_pattn a) {
     const int s = pg_seq_of(a.pool, a.b, r);
     int row0, rows, len;
     if (s < 0 || !pg_seq(a, s, &row0, &rows, &len)) return;
-    const int grp = pg_group_of(a, s), lo = grp >= 0 ? pg_shared(a, grp) : 0;
-    const int parts = pg_parts(len - lo, a.parts), gparts = lo ? pg_parts(lo, a.gparts) : 0;
+    const int lo = pg_prefix_of(a, s);
+    const int parts = pg_parts(len - lo, rows * a.G <= a.few ? a.parts : a.mparts), gparts = lo ? pg_parts(lo, a.gparts) : 0;
     if (parts == 1 && !gparts) return;                 // written already
-    const int64_t at = item * (a.gparts + a.parts);
+    const int64_t at = item * (a.gparts + a.sparts);
     const int np = gparts + parts;
     // part c of np: the prefix's, then the sequence's own
     float M = -INFINITY;
@@ -268,33 +264,27 @@ pattn_join(oh_pattn a) {
 }
 
 template <int RT, int CT, int HD>
-hipError_t go(const oh_pattn *a, hipStream_t st) {
-    const int64_t tiles = ((int64_t)a->b.max_new * a->G + 15) / 16;
-    if (tiles * a->b.n_seq > kMaxBlocks || ((int64_t)a->b.n_rows * a->nh + 3) / 4 > kMaxBlocks) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((pattn_few<RT, CT, HD>), dim3((unsigned)(tiles * a->b.n_seq), a->pool.nkv, a->parts), dim3(256), 0, st, *a, (int)tiles);
-    hipError_t e = hipGetLastError();
-    if (e == hipSuccess && (a->parts > 1 || a->n_group)) {
-        hipLaunchKernelGGL((pattn_join<RT, HD>), dim3((unsigned)(((int64_t)a->b.n_rows * a->nh + 3) / 4)), dim3(256), 0, st, *a);
-        e = hipGetLastError();
+hipError_t go_few(const oh_pattn *a, hipStream_t st) {
+    const int64_t tiles = (std::min((int64_t)a->b.max_new * a->G, (int64_t)a->few) + 15) / 16;
+    if (tiles * a->b.n_seq > kMaxBlocks) return hipErrorInvalidConfiguration;
+    if (a->n_group && !a->gmany) {
+        const int64_t gtiles = ((int64_t)a->b.n_rows * a->G + 15) / 16;
+        if (gtiles * a->n_group > kMaxBlocks) return hipErrorInvalidConfiguration;
+        hipLaunchKernelGGL((pattn_few<RT, CT, HD, true>), dim3((unsigned)(gtiles * a->n_group), a->pool.nkv, a->gparts), dim3(256), 0, st, *a, (int)gtiles);
     }
-    return e;
+    if (tiles)
+        hipLaunchKernelGGL((pattn_few<RT, CT, HD, false>), dim3((unsigned)(tiles * a->b.n_seq), a->pool.nkv, a->parts), dim3(256), 0, st, *a, (int)tiles);
+    return hipGetLastError();
 }
-template <int RT, int CT>
-hipError_t dims(const oh_pattn *a, hipStream_t st) {
-    switch (a->pool.hd) {
-    case 64: return go<RT, CT, 64>(a, st);
-    case 128: return go<RT, CT, 128>(a, st);
-    case 256: return go<RT, CT, 256>(a, st);
-    default: return hipErrorNotSupported;
-    }
+template <int RT, int CT, int HD>
+hipError_t go_join(const oh_pattn *a, hipStream_t st) {
+    const int64_t blocks = ((int64_t)a->b.n_rows * a->nh + 3) / 4;
+    if (blocks > kMaxBlocks) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((pattn_join<RT, HD>), dim3((unsigned)blocks), dim3(256), 0, st, *a);
+    return hipGetLastError();
 }
 
 } // namespace
 
-extern "C" hipError_t oh_launch_paged_attn(const oh_pattn *a, hipStream_t st) {
-    const int r = a->type, c = a->pool.type;
-    if (c == OH_PT_Q8)
-        return r == OH_PT_F32 ? dims<OH_PT_F32, OH_PT_Q8>(a, st) : r == OH_PT_BF16 ? dims<OH_PT_BF16, OH_PT_Q8>(a, st)
-                                                                                    : dims<OH_PT_F16, OH_PT_Q8>(a, st);
-    return c == OH_PT_BF16 ? dims<OH_PT_BF16, OH_PT_BF16>(a, st) : dims<OH_PT_F16, OH_PT_F16>(a, st);
-}
+extern "C" hipError_t oh_launch_pattn_few(const oh_pattn *a, hipStream_t st) { PG_TYPES(go_few, a, st) }
+extern "C" hipError_t oh_launch_pattn_join(const oh_pattn *a, hipStream_t st) { PG_TYPES(go_join, a, st) }

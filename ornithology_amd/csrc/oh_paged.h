@@ -59,16 +59,21 @@ struct oh_pattn {
     oh_pool pool;
     oh_pbatch b;
     oh_prows q, out;
-    float scale;                                // times log2(e): scores are powers of two
+    float scale, sign;                          // |scale| times log2(e): scores are powers of two
     int32_t nh, G, type;
     // shared prefixes: group i: sequences [gfirst[i], gfirst[i + 1]), the
     // whole pages within its glen[i] positions
     const int32_t *gfirst, *glen;
     int32_t n_group;
-    // parts of the key axis: of the sequences, and of the groups' prefixes (at
-    // most; short ones have fewer), and the partial results of row r, head h,
-    // part c at (r * nh + h) * (gparts + parts) + c, the prefix's first
-    int32_t parts, gparts;
+    // Parts of the key axis, at most (short stretches have fewer): of the
+    // sequences that the kernel for few rows takes, of those that the one for
+    // many takes, of the groups' prefixes. The partial result of row r, head h
+    // and part c is at (r * nh + h) * (gparts + sparts) + c, the prefix's
+    // first; sparts = max(parts, mparts)
+    int32_t parts, mparts, gparts, sparts;
+    // sequences of up to `few` rows (times heads of a group) go to the one, of
+    // more than `many` (-1: none) to the other; prefixes by gmany
+    int32_t few, many, gmany;
     float *po;                                  // [..][hd], not divided by the sum
     float2 *pml;                                // [..] running maximum (log2) and sum
 };
@@ -79,5 +84,7 @@ constexpr int64_t kMaxBlocks = (1 << 24) - 1;
 extern "C" {
 hipError_t oh_launch_paged_append(const oh_pappend *a, hipStream_t st);
 hipError_t oh_launch_paged_read(const oh_pappend *a, hipStream_t st);
-hipError_t oh_launch_paged_attn(const oh_pattn *a, hipStream_t st);
+hipError_t oh_launch_pattn_few(const oh_pattn *a, hipStream_t st);    // the sequences' (few) and the prefixes' (not gmany)
+hipError_t oh_launch_pattn_many(const oh_pattn *a, hipStream_t st);   // the sequences' (many) and the prefixes' (gmany)
+hipError_t oh_launch_pattn_join(const oh_pattn *a, hipStream_t st);
 }

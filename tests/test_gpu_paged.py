@@ -172,3 +172,65 @@ def verify(m, q, k, v, out, scale, rows):
 @pytest.mark.parametrize("spec", SPECS, ids=str)
 def test_attend(hip_ctx, rows, cache, hd, nh, nkv, page, spec):
     verify(*run_attention(hip_ctx, rows, cache, hd, nh, nkv, page, SPECS[spec]), None, rows)
+
+
+# ---- shared prefixes --------------------------------------------------------------------
+
+GROUPS = {
+    # rows, lengths, groups' first sequences, prefix
+    "two": ([1, 1], [100, 90], (0, 2), 80),
+    "answers": ([1] * 12, [530 + 3 * i for i in range(12)], (0, 12), 512),
+    "three": ([1] * 20, [300 + 17 * i for i in range(20)], (0, 7, 8, 20), 289),
+    "some": ([1, 2, 1, 40, 3, 1, 9], [333, 700, 290, 512, 257, 80, 20], (1, 5), 256),
+    "pieces": ([130, 1, 64, 77], [900, 770, 900, 860], (0, 4), 768),
+    "short": ([1, 1, 3], [20, 31, 9], (0, 3), 6),
+    "only": ([2, 2, 5], [256, 258, 261], (0, 3), 256),
+}
+
+
+@pytest.mark.parametrize("rows,cache", PAIRS)
+@pytest.mark.parametrize("hd,nh,nkv,page", [(256, 16, 2, 64), (128, 8, 8, 32), (128, 28, 4, 128), (64, 6, 1, 256)])
+@pytest.mark.parametrize("group", GROUPS, ids=str)
+def test_attend_prefix(hip_ctx, rows, cache, hd, nh, nkv, page, group):
+    r, lens, groups, shared = GROUPS[group]
+    verify(*run_attention(hip_ctx, rows, cache, hd, nh, nkv, page, (r, lens), groups=groups, shared=shared), None, rows)
+
+
+# ---- masks --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,cache", PAIRS)
+@pytest.mark.parametrize("hd,nh,nkv,page", [(128, 8, 2, 64), (256, 8, 1, 32), (64, 3, 3, 128)])
+@pytest.mark.parametrize("spec", [([1, 1], [33, 600]), ([9, 3], [40, 200]), ([100], [300]), ([90, 1, 60], [90, 77, 400])], ids=str)
+def test_what_is_hidden_is_not_seen(hip_ctx, rows, cache, hd, nh, nkv, page, spec):
+    """Pages hold another request's infinities and NaN behind a sequence's end,
+    and a prompt's later tokens are infinite or NaN: rows that do not see them
+    are as if they were not there, rows that do are not finite."""
+    g, dt = gen(5), DT[rows]
+    m = Made(*spec, page)
+    pool = hip_ctx.paged_kv(m.n_pages, nkv, hd, page_len=page, type=KV[cache])
+    held = torch.float32 if cache == "q8" else DT[cache]
+    n = m.n_pages
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    every = oa.PagedBatch(i32([page * i for i in range(n + 1)]), i32([page] * n), i32([[i] for i in range(n)]), n_rows=n * page, max_new=page)
+    junk = torch.tensor([math.inf, math.nan, -math.inf, 1.0], device="cuda")[torch.randint(0, 4, (n * page, nkv, hd), generator=g, device="cuda")]
+    pool.append(every, junk.to(held), junk.to(held))
+    k, v = (torch.randn(sum(m.lens), nkv, hd, generator=g, device="cuda").to(held) for _ in range(2))
+    pool.append(m.whole, k, v)
+    q = torch.randn(m.total, nh, hd, generator=g, device="cuda").to(dt)
+    wide = torch.float32 if cache == "q8" else held
+    clean = pool.attend(m.batch, q)
+    verify(m, q, *pool.read(m.whole, wide), clean, None, rows)
+    # the last tokens of every sequence, if they are not all there is
+    bad = [s for s in range(len(m.rows)) if m.rows[s] > 2]
+    for x in (math.nan, math.inf):
+        k2, v2 = k.clone(), v.clone()
+        for s in bad:
+            k2[m.all_start[s + 1] - 1] = math.nan
+            v2[m.all_start[s + 1] - 2:m.all_start[s + 1]] = x
+        pool.append(m.whole, k2, v2)
+        out = pool.attend(m.batch, q)
+        for s in range(len(m.rows)):
+            a, b = m.start[s], m.start[s + 1] - (2 if s in bad else 0)
+            assert torch.equal(out[a:b], clean[a:b])
+            assert not torch.isfinite(out[b:m.start[s + 1]]).any()
+    pool.check()
