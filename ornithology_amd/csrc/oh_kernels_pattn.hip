@@ -15,16 +15,17 @@ template <int RT, int CT, int HD, bool PREFIX>
 __global__ void __launch_bounds__(256)
 pattn_few(oh_pattn a, int tiles_of_rows) {
     typedef typename pg_elem<RT>::t row_t;
-    typedef typename pg_op<CT>::v opv;
-    typedef typename pg_op<CT>::e ope;
+    typedef pg_ops<RT, CT> ops;
+    typedef typename ops::kv kop;
+    typedef typename ops::vv vop;
     constexpr bool Q8 = CT == OH_PT_Q8;
-    constexpr int NQ = pg_nq<RT, CT>(), NP = RT == OH_PT_F32 ? 3 : 2, NS = HD / 32, ND = HD / 16;
+    constexpr int NQ = ops::NQ, NP = RT == OH_PT_F32 ? 3 : 2, NS = HD / 32, ND = HD / 16;
     __shared__ float red[4][16][68];
     __shared__ float sm[4][16], sl[4][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    const int unit = (int)blockIdx.x / tiles_of_rows, rt = (int)blockIdx.x % tiles_of_rows, kvh = blockIdx.y, c = blockIdx.z;
+    const int ui = (int)blockIdx.x / tiles_of_rows, rt = (int)blockIdx.x % tiles_of_rows, kvh = blockIdx.y, c = blockIdx.z;
     pg_unit u;
-    if (!pg_unit_at<PREFIX>(a, unit, &u)) return;
+    if (!pg_unit_at<PREFIX>(a, ui, &u)) return;
     const int G = a.G, F = u.n * G;
     if (rt * 16 >= F || (!PREFIX && F > a.few) || (PREFIX && !u.hi)) return;
     const int parts = pg_parts(u.hi - u.lo, PREFIX ? a.gparts : a.parts);
@@ -37,22 +38,35 @@ pattn_few(oh_pattn a, int tiles_of_rows) {
     const int f = rt * 16 + n, tok = u.row + f / G, head = kvh * G + f % G;
     const bool valid = f < F;
     const int lim = valid ? pg_unit_lim<PREFIX>(a, u, tok) : 0;
-    opv qf[NQ][NS];
+    const row_t *src = (const row_t *)a.q.p + tok * a.q.rs + head * a.q.hs;
+    kop qf[NQ][NS];
+    float unit = a.scale;
+    {
+        float x[NS][8], top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NS; i++) {
-        const int d = Q8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g;
-        float x[8];
+        for (int i = 0; i < NS; i++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = 0.0f;
-        if (valid) {
-            const row_t *src = (const row_t *)a.q.p + tok * a.q.rs + head * a.q.hs + d;
+            for (int j = 0; j < 8; j++) {
+                x[i][j] = valid ? (float)src[(Q8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g) + j] * a.sign : 0.0f;
+                top = fmaxf(top, fabsf(x[i][j]));
+            }
+        if (NQ > 1) {
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const int e = pg_row_exp(top);
+            unit = ldexpf(unit, -e);
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = (float)src[j] * a.sign;
+            for (int i = 0; i < NS; i++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[i][j] = ldexpf(x[i][j], e);
         }
-        opv t[NQ];
-        pg_split<NQ>(x, t);
 #pragma unroll
-        for (int k = 0; k < NQ; k++) qf[k][i] = t[k];
+        for (int i = 0; i < NS; i++) {
+            kop t[NQ];
+            pg_split<NQ>(x[i], t);
+#pragma unroll
+            for (int k = 0; k < NQ; k++) qf[k][i] = t[k];
+        }
     }
     pg_f4 o[ND];
 #pragma unroll
@@ -76,17 +90,19 @@ pattn_few(oh_pattn a, int tiles_of_rows) {
 #pragma unroll
                 for (int i = 0; i < NS / 2; i++) {
                     const uint4 w = *(const uint4 *)(kp + ((4 * i + g) * 32 + 16 * h + n) * 16);
-                    const pg_b8 k0 = pg_codes(w.x, w.y), k1 = pg_codes(w.z, w.w);
+                    kop k0, k1;
+                    pg_codes(w.x, w.y, &k0);
+                    pg_codes(w.z, w.w, &k1);
 #pragma unroll
                     for (int k = NQ - 1; k >= 0; k--) {          // the small terms first
-                        sc[h] = pg_mma16(__builtin_bit_cast(opv, k0), qf[k][2 * i], sc[h]);
-                        sc[h] = pg_mma16(__builtin_bit_cast(opv, k1), qf[k][2 * i + 1], sc[h]);
+                        sc[h] = pg_mma16(k0, qf[k][2 * i], sc[h]);
+                        sc[h] = pg_mma16(k1, qf[k][2 * i + 1], sc[h]);
                     }
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < NS; i++)
-                    sc[h] = pg_mma16(*(const opv *)(kp + ((4 * i + g) * 32 + 16 * h + n) * 16), qf[0][i], sc[h]);
+                    sc[h] = pg_mma16(*(const kop *)(kp + ((4 * i + g) * 32 + 16 * h + n) * 16), qf[0][i], sc[h]);
             }
         }
         float p[8];
@@ -97,7 +113,7 @@ pattn_few(oh_pattn a, int tiles_of_rows) {
             if (Q8) ks = *(const pg_f4 *)(blk + a.pool.ks_off + 4 * (slot + 16 * h + 4 * g));
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float x = Q8 ? sc[h][i] * ks[i] * a.scale : sc[h][i] * a.scale;
+                const float x = Q8 ? sc[h][i] * ks[i] * unit : sc[h][i] * unit;
                 p[4 * h + i] = 16 * h + 4 * g + i < vis ? x : -INFINITY;
                 mx = fmaxf(mx, p[4 * h + i]);
             }
@@ -121,7 +137,7 @@ pattn_few(oh_pattn a, int tiles_of_rows) {
                 p[4 * h + i] = Q8 ? (see ? e * vs[i] : 0.0f) : e;
             }
         }
-        opv pf[NP];
+        vop pf[NP];
         pg_split<NP>(p, pf);
 #pragma unroll
         for (int d = 0; d < ND; d++) o[d] *= alpha;
@@ -130,16 +146,16 @@ pattn_few(oh_pattn a, int tiles_of_rows) {
         // request's leavings, a later token) may be infinite or NaN, and 0
         // times that is NaN: such tiles go row by row, with those values zero
         bool odd = false;
-        opv vf[ND];
+        vop vf[ND];
 #pragma unroll
         for (int d = 0; d < ND; d += 2) {
             if (Q8) {
                 const uint4 w = *(const uint4 *)(vp + (g * HD + 16 * d + 2 * n) * 8);
-                vf[d] = __builtin_bit_cast(opv, pg_codes(w.x, w.y));
-                vf[d + 1] = __builtin_bit_cast(opv, pg_codes(w.z, w.w));
+                pg_codes(w.x, w.y, &vf[d]);
+                pg_codes(w.z, w.w, &vf[d + 1]);
             } else {
-                vf[d] = *(const opv *)(vp + (g * HD + 16 * d + n) * 16);
-                vf[d + 1] = *(const opv *)(vp + (g * HD + 16 * (d + 1) + n) * 16);
+                vf[d] = *(const vop *)(vp + (g * HD + 16 * d + n) * 16);
+                vf[d + 1] = *(const vop *)(vp + (g * HD + 16 * (d + 1) + n) * 16);
             }
         }
         if (!Q8 && __any(valid && vis < 32)) {
@@ -160,9 +176,9 @@ pattn_few(oh_pattn a, int tiles_of_rows) {
                 if (v <= 0) continue;
 #pragma unroll
                 for (int d = 0; d < ND; d++) {
-                    opv x;
+                    vop x;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) x[j] = 16 * (j >> 2) + 4 * g + (j & 3) < v ? vf[d][j] : (ope)0.0f;
+                    for (int j = 0; j < 8; j++) x[j] = 16 * (j >> 2) + 4 * g + (j & 3) < v ? vf[d][j] : (typename ops::ve)0.0f;
                     pg_f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int k = NP - 1; k >= 0; k--) y = pg_mma16(x, pf[k], y);

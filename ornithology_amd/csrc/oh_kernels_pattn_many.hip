@@ -13,33 +13,42 @@
 
 namespace {
 
-constexpr int kT = 64;                                 // positions per step
 // A running maximum may be this much (a factor of 2^8) behind the largest
 // score: weights stay far inside every operand type, 32-bit sums lose nothing,
 // and the accumulators are scaled a few times a row instead of at every step
 constexpr float kBehind = 8.0f;
 
-template <int HD> constexpr int tile_bytes() { return kT * HD * 2; }          // keys, or values, as 16-bit operands
-template <int CT, int HD> constexpr int buf_bytes() { return 2 * tile_bytes<HD>() + (CT == OH_PT_Q8 ? 8 * kT : 0); }
-// waves a block: eight where two fit a SIMD's registers and a step has a load for each thread
-template <int RT, int CT, int HD> constexpr int waves() { return RT == OH_PT_F32 || HD == 256 || (CT == OH_PT_Q8 && HD == 64) ? 4 : 8; }
+// Positions a step, waves a block, and whether the waves take turns: of the two
+// that share a SIMD one has its products while the other has its softmax. That
+// takes eight waves, so two sets of accumulators in a SIMD's registers.
+template <int RT, int CT, int HD> struct many_cfg {
+    static constexpr bool TURNS = RT != OH_PT_F32 && HD < 256 && !(CT == OH_PT_Q8 && HD == 64);
+    static constexpr int T = HD == 256 || (HD == 128 && CT != OH_PT_Q8) ? 32 : 64, NW = TURNS ? 8 : 4, H = T / 32;
+    static constexpr int TILE = T * HD * 2;            // keys, or values, of a step in LDS, as 16-bit operands
+    static constexpr int LDS = 4 * TILE + 2 * (8 * T + 16);   // two of each; scales and whether there is a page
+};
 
-template <int RT, int CT, int HD, bool PREFIX, int NW = waves<RT, CT, HD>()>
-__global__ void __launch_bounds__(64 * NW)
+template <int RT, int CT, int HD, bool PREFIX>
+__global__ void __launch_bounds__((64 * many_cfg<RT, CT, HD>::NW))
 pattn_many(oh_pattn a, int tiles_of_rows) {
     typedef typename pg_elem<RT>::t row_t;
-    typedef typename pg_op<CT>::v opv;
-    typedef typename pg_op<CT>::e ope;
+    typedef pg_ops<RT, CT> ops;
+    typedef typename ops::kv kop;
+    typedef typename ops::vv vop;
+    typedef many_cfg<RT, CT, HD> cfg;
     constexpr bool Q8 = CT == OH_PT_Q8;
-    constexpr int NT = 64 * NW, TR = 32 * NW;
-    constexpr int NQ = pg_nq<RT, CT>(), NP = RT == OH_PT_F32 ? 3 : RT == OH_PT_F16 && Q8 ? 2 : 1, NS = HD / 16, ND = HD / 32;
+    constexpr int NW = cfg::NW, T = cfg::T, H = cfg::H, TILE = cfg::TILE, NT = 64 * NW, TR = 32 * NW;
+    constexpr int NQ = ops::NQ, NP = RT == OH_PT_F32 ? 3 : RT == OH_PT_F16 && Q8 ? 2 : 1, NS = HD / 16, ND = HD / 32;
     extern __shared__ __align__(16) uint8_t lds[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 31, hf = lane >> 5;
+    uint8_t *const ldk = lds, *const ldv = lds + 2 * TILE;
+    float *const lds_s = (float *)(lds + 4 * TILE);    // [2][keys' T, values' T]
+    int *const lds_ok = (int *)(lds_s + 4 * T);        // [2][2]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hf = lane >> 5;
     // long rows first: the last row tiles of a prompt see the most
-    const int unit = (int)blockIdx.x / tiles_of_rows, rt = tiles_of_rows - 1 - (int)blockIdx.x % tiles_of_rows;
+    const int ui = (int)blockIdx.x / tiles_of_rows, rt = tiles_of_rows - 1 - (int)blockIdx.x % tiles_of_rows;
     const int kvh = blockIdx.y, c = blockIdx.z;
     pg_unit u;
-    if (!pg_unit_at<PREFIX>(a, unit, &u)) return;
+    if (!pg_unit_at<PREFIX>(a, ui, &u)) return;
     const int G = a.G, F = u.n * G;
     if (rt * TR >= F || (!PREFIX && F <= a.many) || (PREFIX && !u.hi)) return;
     const int parts = pg_parts(u.hi - u.lo, PREFIX ? a.gparts : a.mparts);
@@ -50,8 +59,8 @@ pattn_many(oh_pattn a, int tiles_of_rows) {
     pg_part(u, c, parts, &t0, &t1);
     const int f = rt * TR + wave * 32 + n, tok = u.row + f / G, head = kvh * G + f % G;
     const bool valid = f < F;
-    int lim = valid ? pg_unit_lim<PREFIX>(a, u, tok) : 0;
-    // the block's and the wave's last visible position
+    // what the lane's row sees of the part; the wave's and the block's last position
+    int lim = valid ? min(pg_unit_lim<PREFIX>(a, u, tok), 32 * t1) : 0;
     int wlim = lim;
 #pragma unroll
     for (int o = 32; o; o >>= 1) wlim = max(wlim, __shfl_xor(wlim, o));
@@ -62,23 +71,37 @@ pattn_many(oh_pattn a, int tiles_of_rows) {
 #pragma unroll
     for (int w = 0; w < NW; w++) blim = max(blim, wl[w]);
     if (!valid) lim = 1 << 30;                         // (no row: nothing to hide)
-    const int p0 = 32 * t0, p1 = min(32 * t1, blim);   // positions [p0, p1), in steps of kT
+    wlim = __builtin_amdgcn_readfirstlane(wlim);
+    blim = __builtin_amdgcn_readfirstlane(blim);
+    const int p0 = 32 * t0, N = blim > p0 ? (blim - p0 + T - 1) / T : 0;       // steps
 
-    opv qf[NQ][NS];
+    kop qf[NQ][NS];
+    float unit = a.scale;                              // of the row's scores as they come out of the products
+    {
+        float x[NS][8], top = 0.0f;
+        const row_t *src = (const row_t *)a.q.p + tok * a.q.rs + head * a.q.hs + 8 * hf;
 #pragma unroll
-    for (int i = 0; i < NS; i++) {
-        float x[8];
+        for (int i = 0; i < NS; i++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = 0.0f;
-        if (valid) {
-            const row_t *src = (const row_t *)a.q.p + tok * a.q.rs + head * a.q.hs + 16 * i + 8 * hf;
+            for (int j = 0; j < 8; j++) {
+                x[i][j] = valid ? (float)src[16 * i + j] * a.sign : 0.0f;
+                top = fmaxf(top, fabsf(x[i][j]));
+            }
+        if (NQ > 1) {
+            const int e = pg_row_exp(fmaxf(top, __shfl_xor(top, 32)));
+            unit = ldexpf(unit, -e);
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = (float)src[j] * a.sign;
+            for (int i = 0; i < NS; i++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[i][j] = ldexpf(x[i][j], e);
         }
-        opv t[NQ];
-        pg_split<NQ>(x, t);
 #pragma unroll
-        for (int k = 0; k < NQ; k++) qf[k][i] = t[k];
+        for (int i = 0; i < NS; i++) {
+            kop t[NQ];
+            pg_split<NQ>(x[i], t);
+#pragma unroll
+            for (int k = 0; k < NQ; k++) qf[k][i] = t[k];
+        }
     }
     pg_f16 o[ND];
 #pragma unroll
@@ -87,214 +110,300 @@ pattn_many(oh_pattn a, int tiles_of_rows) {
         for (int v = 0; v < 16; v++) o[d][v] = 0.0f;
     float m = -INFINITY, l = 0.0f;
 
-    // A step's keys and values: the two 32-position tiles' bytes, 16 a thread
-    // at a time; where there is no page (behind the last position, or a bad
-    // index) the block of page 0, which no row looks at
-    constexpr int KB = 32 * HD * (Q8 ? 1 : 2), NL = 2 * KB / 16 / NT;          // bytes of a tile; loads per thread
-    static_assert(2 * KB == NL * 16 * NT, "whole loads");
+    // ---- a step's keys and values: the 32-position tiles' bytes as they are in
+    // the pool, 16 a thread at a time; where there is no page (behind the last
+    // position, or a bad index) page 0's, which no row looks at
+    constexpr int KB = 32 * HD * (Q8 ? 1 : 2), NL = H * KB / 16 / NT;          // bytes of a tile; loads per thread
+    static_assert(H * KB == NL * 16 * NT, "whole loads");
     uint4 kr[NL], vr[NL];
     float scl = 0.0f;
+    bool ok[H];
     const int page_mask = (1 << a.pool.page_sh) - 1;
-    auto tile_at = [&](int pos, bool *ok) -> const uint8_t * {
+    pg_list lk = {u.pages, a.b.max_pages, 0, 0};
+    lk.hold(p0 >> a.pool.page_sh);
+    pg_list lv = lk;
+    bool bad = false;
+    auto tile_at = [&](pg_list &list, int pos, bool *there) -> const uint8_t * {
         int page = -1;
-        if (pos < p1) {
-            page = u.pages[pos >> a.pool.page_sh];
-            if (page < 0 || page >= a.pool.n_pages) { page = -1; if (tid == 0) pg_report(a.pool, OH_PF_PAGE); }
+        if (pos < blim) {
+            page = list.get(pos >> a.pool.page_sh);
+            if (page < 0 || page >= a.pool.n_pages) { page = -1; bad = true; }
         }
-        *ok = page >= 0;
-        return pg_block(a.pool, page < 0 ? 0 : page, kvh);
+        *there = page >= 0;
+        return pg_block(a.pool, page < 0 ? 0 : page, kvh) + (size_t)((pos & page_mask) >> 5) * KB;
     };
-    const uint8_t *blk[2];
-    bool ok[2];
-    auto fetch = [&](int pos) {
+    auto fetch = [&](pg_list &list, int pos, uint32_t plane, uint4 (&r)[NL], bool keys = false) {
+        const uint8_t *at[H];
+        bool there[H];
 #pragma unroll
-        for (int h = 0; h < 2; h++) blk[h] = tile_at(pos + 32 * h, &ok[h]);
+        for (int h = 0; h < H; h++) at[h] = tile_at(list, pos + 32 * h, &there[h]);
 #pragma unroll
         for (int i = 0; i < NL; i++) {
-            const int b = (tid + NT * i) * 16, h = b / KB, off = b % KB;
-            const uint8_t *from = blk[h] + ((pos + 32 * h) & page_mask) / 32 * KB + off;
-            kr[i] = *(const uint4 *)from;
-            vr[i] = *(const uint4 *)(from + a.pool.v_off);
+            const int b = (tid + NT * i) * 16;
+            r[i] = ldg((const uint4 *)((H == 1 || b < KB ? at[0] : at[H - 1]) + plane + b % KB));
         }
-        if (Q8 && tid < 2 * kT) {
-            const int x = tid & (kT - 1), h = x >> 5;
-            scl = *(const float *)(blk[h] + (tid < kT ? a.pool.ks_off : a.pool.vs_off) + 4 * ((pos + x) & page_mask));
+        if (keys)
+#pragma unroll
+            for (int h = 0; h < H; h++) ok[h] = there[h];
+        if (keys && Q8 && tid < 2 * T) {
+            const int x = tid & (T - 1), p = pos + x;
+            const uint8_t *blk = (x < 32 ? at[0] : at[H - 1]) - (size_t)((p & page_mask) >> 5) * KB;
+            scl = ldg((const float *)(blk + (tid < T ? a.pool.ks_off : a.pool.vs_off) + 4 * (p & page_mask)));
         }
     };
-    // into buffer b: K units (8 dims of one position) at (dim / 8 * 32 +
-    // position) * 16 per tile, V units (8 positions of one dim) at (group * HD + dim) * 16
-    auto stage = [&](int b) {
-        uint8_t *K = lds + b * buf_bytes<CT, HD>(), *V = K + tile_bytes<HD>();
+    // keys: units (8 dims of one position) at (dim / 8 * 32 + position) * 16 of a
+    // tile; values: units (8 positions of one dim) at (group * HD + dim) * 16
+    auto stage_k = [&](int b) {
 #pragma unroll
         for (int i = 0; i < NL; i++) {
             const int e = tid + NT * i;
             if (Q8) {
                 const int h = e * 16 / KB, x = e % (KB / 16), ch = x >> 5, sl = x & 31;      // 16 dims ch of position sl
-                uint8_t *kt = K + h * 64 * HD;
-                *(pg_b8 *)(kt + ((2 * ch) * 32 + sl) * 16) = pg_codes(kr[i].x, kr[i].y);
-                *(pg_b8 *)(kt + ((2 * ch + 1) * 32 + sl) * 16) = pg_codes(kr[i].z, kr[i].w);
-                *(pg_b8 *)(V + e * 32) = pg_codes(vr[i].x, vr[i].y);
-                *(pg_b8 *)(V + e * 32 + 16) = pg_codes(vr[i].z, vr[i].w);
+                kop *to = (kop *)(ldk + b * TILE + h * 64 * HD) + 2 * ch * 32 + sl;
+                kop k0, k1;
+                pg_codes(kr[i].x, kr[i].y, &k0);
+                pg_codes(kr[i].z, kr[i].w, &k1);
+                to[0] = k0;
+                to[32] = k1;
             } else {
-                *(uint4 *)(K + e * 16) = kr[i];
-                *(uint4 *)(V + e * 16) = vr[i];
+                *(uint4 *)(ldk + b * TILE + e * 16) = kr[i];
             }
         }
-        if (Q8 && tid < 2 * kT) *(float *)(K + 2 * tile_bytes<HD>() + 4 * tid) = tid < kT ? scl * a.scale : scl;
+        if (Q8 && tid < 2 * T) lds_s[b * 2 * T + tid] = scl;
+        if (tid == 0)
+#pragma unroll
+            for (int h = 0; h < H; h++) lds_ok[2 * b + h] = ok[h];
+    };
+    auto stage_v = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const int e = tid + NT * i;
+            if (Q8) {
+                vop v0, v1;
+                pg_codes(vr[i].x, vr[i].y, &v0);
+                pg_codes(vr[i].z, vr[i].w, &v1);
+                vop *to = (vop *)(ldv + b * TILE) + 2 * e;
+                to[0] = v0;
+                to[1] = v1;
+            } else {
+                *(uint4 *)(ldv + b * TILE + e * 16) = vr[i];
+            }
+        }
     };
 
-    bool now[2];
-    if (p0 < p1) {
-        fetch(p0);
-        stage(0);
-    }
-    int b = 0;
-    for (int pos = p0; pos < p1; pos += kT, b ^= 1) {
-        now[0] = ok[0]; now[1] = ok[1];
-        __syncthreads();                               // buffer b is whole, the other one free
-        const bool more = pos + kT < p1;
-        if (more) fetch(pos + kT);
-        if (pos < wlim) {
-            const uint8_t *K = lds + b * buf_bytes<CT, HD>(), *V = K + tile_bytes<HD>();
-            const float *ks = (const float *)(K + 2 * tile_bytes<HD>()), *vs = ks + kT;
-            pg_f16 s[2];
+    // ---- products: S^T of step t, and O^T of the step before
+    pg_f16 s[H];
+    vop pf[NP][H][2];
+    int vis[H];                                        // of the step whose weights are in pf
+    bool part = false;                                 // some row sees a part of it only
+    auto scores = [&](int t) {
+        // operand row n is position 16 (n >> 3 & 1) + 8 (n >> 4) + (n & 7), so that
+        // a lane's 8 scores of a product are one unit of the values
+        const kop *at = (const kop *)(ldk + (t & 1) * TILE) + hf * 32 + 16 * ((n >> 3) & 1) + 8 * (n >> 4) + (n & 7);
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
+        for (int h = 0; h < H; h++) {
 #pragma unroll
-                for (int v = 0; v < 16; v++) s[h][v] = 0.0f;
-                // operand row n is position 16 (n >> 3 & 1) + 8 (n >> 4) + (n & 7), so that
-                // a lane's 8 scores of a product are one unit of the values
-                const uint8_t *at = K + h * 64 * HD + (hf * 32 + 16 * ((n >> 3) & 1) + 8 * (n >> 4) + (n & 7)) * 16;
+            for (int v = 0; v < 16; v++) s[h][v] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < NS; i++) {
-                    const opv kf = *(const opv *)(at + i * 1024);
+            for (int i = 0; i < NS; i++) {
+                const kop kf = at[h * 4 * HD + i * 64];
 #pragma unroll
-                    for (int k = NQ - 1; k >= 0; k--) s[h] = pg_mma32(kf, qf[k][i], s[h]);
-                }
-            }
-            // scores in units of log2(e), those that the row does not see at -inf
-            const int vis0 = now[0] ? lim - pos : 0, vis1 = now[1] ? lim - pos - 32 : 0;     // visible ones of each tile
-            const bool part = __any(vis0 < 32 || vis1 < 32);
-            if (Q8) {
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        const pg_f4 kk = *(const pg_f4 *)(ks + 32 * h + 16 * (q & 1) + 8 * (q >> 1) + 4 * hf);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) s[h][4 * q + i] *= kk[i];
-                    }
-            }
-            if (part) {
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int v = 0; v < 16; v++)
-                        if (16 * ((v >> 2) & 1) + 8 * (v >> 3) + 4 * hf + (v & 3) >= (h ? vis1 : vis0)) s[h][v] = -INFINITY;
-            }
-            const float unit_scale = Q8 ? 1.0f : a.scale;        // (codes: in their scales)
-            float mx = -INFINITY;
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int v = 0; v < 16; v++) mx = fmaxf(mx, s[h][v]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32)) * unit_scale;
-            if (__any(mx > m + kBehind)) {
-                const float mn = fmaxf(m, mx), alpha = mn == m ? 1.0f : pg_exp2(m - mn);
-                m = mn;
-                l *= alpha;
-#pragma unroll
-                for (int d = 0; d < ND; d++)
-#pragma unroll
-                    for (int v = 0; v < 16; v++) o[d][v] *= alpha;
-            }
-            const float ref = m == -INFINITY ? 0.0f : m;         // (nothing seen yet, or keys of -inf)
-            opv pf[NP][2][2];
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    float p[8];
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        p[j] = pg_exp2(fmaf(s[h][8 * k + j], unit_scale, -ref));
-                        l += p[j];
-                    }
-                    if (Q8) {
-#pragma unroll
-                        for (int q = 0; q < 2; q++) {
-                            const pg_f4 vv = *(const pg_f4 *)(vs + 32 * h + 16 * q + 8 * k + 4 * hf);
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                // (a scale that the row does not see may be anything)
-                                const bool see = !part || 16 * q + 8 * k + 4 * hf + i < (h ? vis1 : vis0);
-                                p[4 * q + i] = see ? p[4 * q + i] * vv[i] : 0.0f;
-                            }
-                        }
-                    }
-                    opv t[NP];
-                    pg_split<NP>(p, t);
-#pragma unroll
-                    for (int x = 0; x < NP; x++) pf[x][h][k] = t[x];
-                }
-            // In a tile that some row sees a part of, values that are hidden from it
-            // may be infinite or NaN, and 0 times that is NaN
-            bool odd = false;
-            if (!Q8 && part) {
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int d = 0; d < ND; d++)
-#pragma unroll
-                        for (int k = 0; k < 2; k++) {
-                            const opv vf = *(const opv *)(V + h * 64 * HD + ((2 * k + hf) * HD + 32 * d + n) * 16);
-#pragma unroll
-                            for (int j = 0; j < 8; j++) odd |= !isfinite((float)vf[j]);
-                        }
-                odd = __any(odd);
-            }
-            if (!odd) {
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int k = 0; k < 2; k++)
-#pragma unroll
-                        for (int d = 0; d < ND; d++) {
-                            const opv vf = *(const opv *)(V + h * 64 * HD + ((2 * k + hf) * HD + 32 * d + n) * 16);
-#pragma unroll
-                            for (int x = NP - 1; x >= 0; x--) o[d] = pg_mma32(vf, pf[x][h][k], o[d]);
-                        }
-            } else {
-                // row by row, with what the row does not see as zero
-#pragma unroll 1
-                for (int r = 0; r < 32; r++) {
-                    const int v0 = __shfl(vis0, r), v1 = __shfl(vis1, r);
-                    asm volatile("" ::: "memory");               // (the values are read where they are used, not kept)
-#pragma unroll
-                    for (int d = 0; d < ND; d++) {
-                        pg_f16 y;
-#pragma unroll
-                        for (int v = 0; v < 16; v++) y[v] = 0.0f;
-#pragma unroll
-                        for (int h = 0; h < 2; h++)
-#pragma unroll
-                            for (int k = 0; k < 2; k++) {
-                                opv vf = *(const opv *)(V + h * 64 * HD + ((2 * k + hf) * HD + 32 * d + n) * 16);
-#pragma unroll
-                                for (int j = 0; j < 8; j++)
-                                    if (16 * (j >> 2) + 8 * k + 4 * hf + (j & 3) >= (h ? v1 : v0)) vf[j] = (ope)0.0f;
-#pragma unroll
-                                for (int x = NP - 1; x >= 0; x--) y = pg_mma32(vf, pf[x][h][k], y);
-                            }
-                        if (n == r)
-#pragma unroll
-                            for (int v = 0; v < 16; v++) o[d][v] += y[v];
-                    }
-                }
+                for (int k = NQ - 1; k >= 0; k--) s[h] = pg_mma32(kf, qf[k][i], s[h]);       // the small term first
             }
         }
-        if (more) stage(b ^ 1);
+    };
+    auto values = [&](int t) {
+        const vop *at = (const vop *)(ldv + (t & 1) * TILE) + hf * HD + n;
+        auto unit_at = [&](int h, int k, int d) { return at[h * 4 * HD + 2 * k * HD + 32 * d]; };
+        // In a step that some row sees a part of, values that are hidden from it
+        // may be infinite or NaN, and 0 times that is NaN
+        bool odd = false;
+        if (!Q8 && part) {
+#pragma unroll 1
+            for (int x = 0; x < 2 * H * ND; x++) {
+                const vop vf = unit_at(x / (2 * ND), x / ND & 1, x % ND);
+#pragma unroll
+                for (int j = 0; j < 8; j++) odd |= !isfinite((float)vf[j]);
+            }
+            odd = __any(odd);
+        }
+        if (__builtin_expect(!odd, 1)) {
+#pragma unroll
+            for (int h = 0; h < H; h++)
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int d = 0; d < ND; d++) {
+                        const vop vf = unit_at(h, k, d);
+#pragma unroll
+                        for (int x = NP - 1; x >= 0; x--) o[d] = pg_mma32(vf, pf[x][h][k], o[d]);
+                    }
+            return;
+        }
+        // row by row, with what the row does not see as zero
+#pragma unroll 1
+        for (int r = 0; r < 32; r++) {
+            asm volatile("" ::: "memory");             // (the values are read where they are used, not kept)
+            int see[H];                                // (of positions counted from the lane's first)
+#pragma unroll
+            for (int h = 0; h < H; h++) see[h] = __builtin_amdgcn_readlane(vis[h], r) - 4 * hf;
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                pg_f16 y;
+#pragma unroll
+                for (int v = 0; v < 16; v++) y[v] = 0.0f;
+#pragma unroll
+                for (int h = 0; h < H; h++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        vop vf = unit_at(h, k, d);
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            if (16 * (j >> 2) + 8 * k + (j & 3) >= see[h]) vf[j] = (typename ops::ve)0.0f;
+#pragma unroll
+                        for (int x = NP - 1; x >= 0; x--) y = pg_mma32(vf, pf[x][h][k], y);
+                    }
+                if (n == r)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) o[d][v] += y[v];
+            }
+        }
+    };
+
+    // ---- the softmax of step t: weights from scores
+    auto softmax = [&](int t) {
+        const int pos = p0 + t * T, b = t & 1;
+        const float *ks = lds_s + b * 2 * T, *vs = ks + T;
+        bool some = false;
+#pragma unroll
+        for (int h = 0; h < H; h++) {
+            vis[h] = __builtin_amdgcn_readfirstlane(lds_ok[2 * b + h]) ? lim - pos - 32 * h : 0;
+            some |= vis[h] < 32;
+        }
+        part = __any(some);
+        if (Q8) {
+#pragma unroll
+            for (int h = 0; h < H; h++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const pg_f4 kk = *(const pg_f4 *)(ks + 32 * h + 16 * (q & 1) + 8 * (q >> 1) + 4 * hf);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[h][4 * q + i] *= kk[i];
+                }
+        }
+        if (part) {
+#pragma unroll
+            for (int h = 0; h < H; h++)
+#pragma unroll
+                for (int v = 0; v < 16; v++)
+                    if (16 * ((v >> 2) & 1) + 8 * (v >> 3) + (v & 3) >= vis[h] - 4 * hf) s[h][v] = -INFINITY;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < H; h++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) mx = fmaxf(mx, s[h][v]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32)) * unit;
+        if (__any(mx > m + kBehind)) {
+            const float mn = fmaxf(m, mx), alpha = mn == m ? 1.0f : pg_exp2(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int v = 0; v < 16; v++) o[d][v] *= alpha;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;   // (nothing seen yet, or keys of -inf)
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int h = 0; h < H; h++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                float p[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    p[j] = pg_exp2(fmaf(s[h][8 * k + j], unit, -ref));
+                    sum[j & 3] += p[j];
+                }
+                if (Q8) {
+#pragma unroll
+                    for (int q = 0; q < 2; q++) {
+                        const pg_f4 vv = *(const pg_f4 *)(vs + 32 * h + 16 * q + 8 * k + 4 * hf);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            // (a scale that the row does not see may be anything)
+                            const bool see = !part || 16 * q + 8 * k + i < vis[h] - 4 * hf;
+                            p[4 * q + i] = see ? p[4 * q + i] * vv[i] : 0.0f;
+                        }
+                    }
+                }
+                vop w[NP];
+                pg_split<NP>(p, w);
+#pragma unroll
+                for (int x = 0; x < NP; x++) pf[x][h][k] = w[x];
+            }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    };
+
+    // Loads and products run one step past the end, on page 0's bytes and for
+    // nothing: no branch splits the loops' registers.
+    fetch(lk, p0, 0, kr, true);
+    if (!cfg::TURNS) fetch(lv, p0, a.pool.v_off, vr);
+    stage_k(0);
+    if (!cfg::TURNS) stage_v(0);
+    __syncthreads();
+    if (!cfg::TURNS) {
+        for (int t = 0; t < N; t++) {
+            fetch(lk, p0 + (t + 1) * T, 0, kr, true);
+            fetch(lv, p0 + (t + 1) * T, a.pool.v_off, vr);
+            scores(t);
+            softmax(t);
+            values(t);
+            stage_k(~t & 1);
+            stage_v(~t & 1);
+            __syncthreads();
+        }
+    } else {
+        // Half-steps, a barrier after each. The first four waves have their
+        // products (O of step t - 1, S of step t) in half-step 2t and the softmax of
+        // t in 2t + 1; the others half a step later. Half-step 2t requests the keys
+        // of step t + 1 and the values of t; 2t + 1 puts them where those of two
+        // steps before were, whose last readers were done in half-step 2t - 1.
+        fetch(lv, p0, a.pool.v_off, vr);
+        fetch(lk, p0 + T, 0, kr, true);
+        if (wave < NW / 2) {
+            scores(0);
+            __syncthreads();
+            for (int t = 0; t < N; t++) {
+                softmax(t);
+                stage_v(t & 1);
+                stage_k(~t & 1);
+                __syncthreads();
+                fetch(lv, p0 + (t + 1) * T, a.pool.v_off, vr);
+                fetch(lk, p0 + (t + 2) * T, 0, kr, true);
+                values(t);
+                scores(t + 1);
+                __syncthreads();
+            }
+        } else {
+            __syncthreads();
+            scores(0);
+            stage_v(0);
+            stage_k(1);
+            for (int t = 0; t < N; t++) {
+                __syncthreads();
+                fetch(lv, p0 + (t + 1) * T, a.pool.v_off, vr);
+                fetch(lk, p0 + (t + 2) * T, 0, kr, true);
+                softmax(t);
+                __syncthreads();
+                values(t);
+                scores(t + 1);
+                stage_v(~t & 1);
+                stage_k(t & 1);
+            }
+        }
     }
+    if (bad && tid == 0) pg_report(a.pool, OH_PF_PAGE);
     l += __shfl_xor(l, 32);
     if (l != l) m = fmaxf(m, 0.0f);                    // a NaN score stays one
     if (!valid) return;
@@ -325,7 +434,7 @@ pattn_many(oh_pattn a, int tiles_of_rows) {
 
 template <int RT, int CT, int HD, bool PREFIX>
 hipError_t launch(const oh_pattn *a, int64_t rows, int units, int parts, hipStream_t st) {
-    constexpr int NW = waves<RT, CT, HD>(), lds = 2 * buf_bytes<CT, HD>();
+    constexpr int NW = many_cfg<RT, CT, HD>::NW, lds = many_cfg<RT, CT, HD>::LDS;
     const int64_t tiles = (rows * a->G + 32 * NW - 1) / (32 * NW);
     if (tiles * units > kMaxBlocks / 2) return hipErrorInvalidConfiguration;
     const auto k = pattn_many<RT, CT, HD, PREFIX>;

@@ -4,20 +4,26 @@
 // o = sum_{t < lim} softmax_t(q . k_t * scale) v_t per row and head, lim the
 // row's position + 1. Scores are taken in units of log2(e), so that the
 // softmax is 2^(s - m). Products run on the matrix cores with 32-bit
-// accumulators; rows of 32 bits (and 16-bit fp rows over codes) enter as sums
-// of bf16 terms, whose products with the codes are exact: three terms hold 24
-// bits, so nothing of an f32 row is lost.
+// accumulators; f32 rows enter as sums of 16-bit terms, whose products with the
+// codes are exact, and their weights as three bf16 terms (24 bits).
 #pragma once
 #include "oh_paged_dev.h"
 
-// operand vectors of the matrix instructions: fp16 for fp16 pools, else bf16
-// (codes up to 127 are exact in either; bf16 has f32's range, so a weight
-// p * scale cannot leave it)
-template <int CT> struct pg_op { typedef pg_b8 v; typedef __bf16 e; };
-template <> struct pg_op<OH_PT_F16> { typedef pg_h8 v; typedef _Float16 e; };
-
-// terms of a query, and of a probability (times its value's scale)
-template <int RT, int CT> constexpr int pg_nq() { return RT == OH_PT_F32 ? 3 : RT == OH_PT_F16 && CT == OH_PT_Q8 ? 2 : 1; }
+// Operand vectors of the matrix instructions. Of the values: fp16 for fp16
+// pools, else bf16, which has f32's range, so that a weight p * scale cannot
+// leave it; codes are exact in either. Of the keys the same, but fp16 over
+// codes for f32 and fp16 rows: two fp16 terms hold 22 bits of a query (scaled so
+// that its largest dim is 2^14 or more, every dim above 2^-17 of that one
+// does), one an fp16 query whole.
+template <bool H> struct pg_vec { typedef pg_b8 v; typedef __bf16 e; };
+template <> struct pg_vec<true> { typedef pg_h8 v; typedef _Float16 e; };
+template <int RT, int CT> struct pg_ops {
+    static constexpr bool Q8 = CT == OH_PT_Q8, KH = CT == OH_PT_F16 || (Q8 && RT != OH_PT_BF16), VH = CT == OH_PT_F16;
+    typedef typename pg_vec<KH>::v kv;
+    typedef typename pg_vec<VH>::v vv;
+    typedef typename pg_vec<VH>::e ve;
+    static constexpr int NQ = RT == OH_PT_F32 ? 2 : 1;
+};
 
 OH_DEV pg_f4 pg_mma16(pg_b8 a, pg_b8 b, pg_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 OH_DEV pg_f4 pg_mma16(pg_h8 a, pg_h8 b, pg_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -39,12 +45,25 @@ OH_DEV void pg_split(const float (&x)[8], V (&out)[N]) {
         }
 }
 // 8 codes as operand values
-OH_DEV pg_b8 pg_codes(uint32_t lo, uint32_t hi) {
-    pg_b8 o;
+OH_DEV void pg_codes(uint32_t lo, uint32_t hi, pg_b8 *o) {
 #pragma unroll
-    for (int j = 0; j < 8; j++) o[j] = (__bf16)(float)(int8_t)((j < 4 ? lo : hi) >> (8 * (j & 3)));
-    return o;
+    for (int j = 0; j < 8; j++) (*o)[j] = (__bf16)(float)(int8_t)((j < 4 ? lo : hi) >> (8 * (j & 3)));
 }
+// (fp16: code + 128 under the exponent of 1024 is 1152 + code)
+OH_DEV void pg_codes(uint32_t lo, uint32_t hi, pg_h8 *o) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    lo ^= 0x80808080u;
+    hi ^= 0x80808080u;
+    const h2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+    const h2 a = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, lo, 0x04010400u)) - off,
+             b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, lo, 0x04030402u)) - off,
+             c = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, hi, 0x04010400u)) - off,
+             d = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, hi, 0x04030402u)) - off;
+    *o = (pg_h8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// The power of two by which a row whose largest |value| is `top` is multiplied
+// before it is split into fp16 terms: top becomes 2^14 or more, below 2^15
+OH_DEV int pg_row_exp(float top) { return top > 0.0f && top < INFINITY ? 14 - max(ilogbf(top), -100) : 0; }
 
 // ---- the batch ------------------------------------------------------------------
 // sequence s's rows and length, false (and reported) if they are not in range
@@ -111,6 +130,23 @@ OH_DEV int pg_unit_lim(const oh_pattn &a, const pg_unit &u, int token) {
     const int lim = pg_lim(len, row + n, token);
     return lim < u.hi ? lim : u.hi;
 }
+
+// A page list in a wave's registers, 64 entries at a time: an entry is a lane of
+// one, where a load of its own would put a round trip to memory before every
+// tile's loads
+struct pg_list {
+    const int32_t *pages;
+    int n, first, mine;                                // entries, the first held one, this lane's
+    OH_DEV void hold(int i) {
+        first = i;
+        const int at = i + (int)(threadIdx.x & 63);
+        mine = at < n ? pages[at] : -1;
+    }
+    OH_DEV int get(int i) {                            // i: the same in the whole wave, never falling
+        if (i - first >= 64) hold(i);
+        return __builtin_amdgcn_readlane(mine, i - first);
+    }
+};
 
 // parts of a stretch of n positions: at most `most`, of at least 4 tiles each
 // (a part's partial result is as large as two positions of a 16-bit pool)
