@@ -23,7 +23,7 @@ constexpr float kBehind = 8.0f;
 // takes eight waves, so two sets of accumulators in a SIMD's registers.
 template <int RT, int CT, int HD> struct many_cfg {
     static constexpr bool TURNS = RT != OH_PT_F32 && HD < 256 && !(CT == OH_PT_Q8 && HD == 64);
-    static constexpr int T = HD == 256 || (HD == 128 && CT != OH_PT_Q8) ? 32 : 64, NW = TURNS ? 8 : 4, H = T / 32;
+    static constexpr int T = HD == 256 ? 32 : 64, NW = TURNS ? 8 : 4, H = T / 32;
     static constexpr int TILE = T * HD * 2;            // keys, or values, of a step in LDS, as 16-bit operands
     static constexpr int LDS = 4 * TILE + 2 * (8 * T + 16);   // two of each; scales and whether there is a page
 };
@@ -59,20 +59,23 @@ pattn_many(oh_pattn a, int tiles_of_rows) {
     pg_part(u, c, parts, &t0, &t1);
     const int f = rt * TR + wave * 32 + n, tok = u.row + f / G, head = kvh * G + f % G;
     const bool valid = f < F;
-    // what the lane's row sees of the part; the wave's and the block's last position
+    // what the lane's row sees of the part; the last position that some row of the
+    // block sees, and the first that some row does not
     int lim = valid ? min(pg_unit_lim<PREFIX>(a, u, tok), 32 * t1) : 0;
-    int wlim = lim;
+    int blim = lim, bmin = valid ? lim : 1 << 30;
 #pragma unroll
-    for (int o = 32; o; o >>= 1) wlim = max(wlim, __shfl_xor(wlim, o));
-    __shared__ int wl[NW];
-    if (lane == 0) wl[wave] = wlim;
+    for (int o = 32; o; o >>= 1) {
+        blim = max(blim, __shfl_xor(blim, o));
+        bmin = min(bmin, __shfl_xor(bmin, o));
+    }
+    __shared__ int wl[2][NW];
+    if (lane == 0) { wl[0][wave] = blim; wl[1][wave] = bmin; }
     __syncthreads();
-    int blim = 0;
 #pragma unroll
-    for (int w = 0; w < NW; w++) blim = max(blim, wl[w]);
+    for (int w = 0; w < NW; w++) { blim = max(blim, wl[0][w]); bmin = min(bmin, wl[1][w]); }
     if (!valid) lim = 1 << 30;                         // (no row: nothing to hide)
-    wlim = __builtin_amdgcn_readfirstlane(wlim);
     blim = __builtin_amdgcn_readfirstlane(blim);
+    bmin = __builtin_amdgcn_readfirstlane(bmin);
     const int p0 = 32 * t0, N = blim > p0 ? (blim - p0 + T - 1) / T : 0;       // steps
 
     kop qf[NQ][NS];
@@ -132,6 +135,7 @@ pattn_many(oh_pattn a, int tiles_of_rows) {
         *there = page >= 0;
         return pg_block(a.pool, page < 0 ? 0 : page, kvh) + (size_t)((pos & page_mask) >> 5) * KB;
     };
+    bool odd = false, hide = false;                    // (hide: of the step whose values are in vr)
     auto fetch = [&](pg_list &list, int pos, uint32_t plane, uint4 (&r)[NL], bool keys = false) {
         const uint8_t *at[H];
         bool there[H];
@@ -142,9 +146,14 @@ pattn_many(oh_pattn a, int tiles_of_rows) {
             const int b = (tid + NT * i) * 16;
             r[i] = ldg((const uint4 *)((H == 1 || b < KB ? at[0] : at[H - 1]) + plane + b % KB));
         }
-        if (keys)
+        if (keys) {
 #pragma unroll
             for (int h = 0; h < H; h++) ok[h] = there[h];
+        } else {
+            hide = pos + T > bmin;
+#pragma unroll
+            for (int h = 0; h < H; h++) hide |= !there[h];
+        }
         if (keys && Q8 && tid < 2 * T) {
             const int x = tid & (T - 1), p = pos + x;
             const uint8_t *blk = (x < 32 ? at[0] : at[H - 1]) - (size_t)((p & page_mask) >> 5) * KB;
@@ -175,6 +184,9 @@ pattn_many(oh_pattn a, int tiles_of_rows) {
             for (int h = 0; h < H; h++) lds_ok[2 * b + h] = ok[h];
     };
     auto stage_v = [&](int b) {
+        if (!Q8 && hide)
+#pragma unroll
+            for (int i = 0; i < NL; i++) pg_only_finite<ops::VH>(&vr[i], &odd);
 #pragma unroll
         for (int i = 0; i < NL; i++) {
             const int e = tid + NT * i;
@@ -194,8 +206,6 @@ pattn_many(oh_pattn a, int tiles_of_rows) {
     // ---- products: S^T of step t, and O^T of the step before
     pg_f16 s[H];
     vop pf[NP][H][2];
-    int vis[H];                                        // of the step whose weights are in pf
-    bool part = false;                                 // some row sees a part of it only
     auto scores = [&](int t) {
         // operand row n is position 16 (n >> 3 & 1) + 8 (n >> 4) + (n & 7), so that
         // a lane's 8 scores of a product are one unit of the values
@@ -215,72 +225,30 @@ pattn_many(oh_pattn a, int tiles_of_rows) {
     auto values = [&](int t) {
         const vop *at = (const vop *)(ldv + (t & 1) * TILE) + hf * HD + n;
         auto unit_at = [&](int h, int k, int d) { return at[h * 4 * HD + 2 * k * HD + 32 * d]; };
-        // In a step that some row sees a part of, values that are hidden from it
-        // may be infinite or NaN, and 0 times that is NaN
-        bool odd = false;
-        if (!Q8 && part) {
-#pragma unroll 1
-            for (int x = 0; x < 2 * H * ND; x++) {
-                const vop vf = unit_at(x / (2 * ND), x / ND & 1, x % ND);
 #pragma unroll
-                for (int j = 0; j < 8; j++) odd |= !isfinite((float)vf[j]);
-            }
-            odd = __any(odd);
-        }
-        if (__builtin_expect(!odd, 1)) {
+        for (int h = 0; h < H; h++)
 #pragma unroll
-            for (int h = 0; h < H; h++)
+            for (int k = 0; k < 2; k++)
 #pragma unroll
-                for (int k = 0; k < 2; k++)
+                for (int d = 0; d < ND; d++) {
+                    const vop vf = unit_at(h, k, d);
 #pragma unroll
-                    for (int d = 0; d < ND; d++) {
-                        const vop vf = unit_at(h, k, d);
-#pragma unroll
-                        for (int x = NP - 1; x >= 0; x--) o[d] = pg_mma32(vf, pf[x][h][k], o[d]);
-                    }
-            return;
-        }
-        // row by row, with what the row does not see as zero
-#pragma unroll 1
-        for (int r = 0; r < 32; r++) {
-            asm volatile("" ::: "memory");             // (the values are read where they are used, not kept)
-            int see[H];                                // (of positions counted from the lane's first)
-#pragma unroll
-            for (int h = 0; h < H; h++) see[h] = __builtin_amdgcn_readlane(vis[h], r) - 4 * hf;
-#pragma unroll
-            for (int d = 0; d < ND; d++) {
-                pg_f16 y;
-#pragma unroll
-                for (int v = 0; v < 16; v++) y[v] = 0.0f;
-#pragma unroll
-                for (int h = 0; h < H; h++)
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        vop vf = unit_at(h, k, d);
-#pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            if (16 * (j >> 2) + 8 * k + (j & 3) >= see[h]) vf[j] = (typename ops::ve)0.0f;
-#pragma unroll
-                        for (int x = NP - 1; x >= 0; x--) y = pg_mma32(vf, pf[x][h][k], y);
-                    }
-                if (n == r)
-#pragma unroll
-                    for (int v = 0; v < 16; v++) o[d][v] += y[v];
-            }
-        }
+                    for (int x = NP - 1; x >= 0; x--) o[d] = pg_mma32(vf, pf[x][h][k], o[d]);
+                }
     };
 
     // ---- the softmax of step t: weights from scores
     auto softmax = [&](int t) {
         const int pos = p0 + t * T, b = t & 1;
         const float *ks = lds_s + b * 2 * T, *vs = ks + T;
+        int vis[H];                                    // positions of a tile below this are visible to the row
         bool some = false;
 #pragma unroll
         for (int h = 0; h < H; h++) {
             vis[h] = __builtin_amdgcn_readfirstlane(lds_ok[2 * b + h]) ? lim - pos - 32 * h : 0;
             some |= vis[h] < 32;
         }
-        part = __any(some);
+        const bool part = __any(some);
         if (Q8) {
 #pragma unroll
             for (int h = 0; h < H; h++)
@@ -404,6 +372,21 @@ pattn_many(oh_pattn a, int tiles_of_rows) {
         }
     }
     if (bad && tid == 0) pg_report(a.pool, OH_PF_PAGE);
+    if (!Q8 && __syncthreads_or(odd)) {
+        // dims 32 d + 8 q + 4 hf + i of the lane's row
+        for (int p = max(p0, bmin); p < blim; p++) {
+            const int page = u.pages[p >> a.pool.page_sh];
+            if (p >= lim || !valid || page < 0 || page >= a.pool.n_pages) continue;
+            const typename ops::ve *at = (const typename ops::ve *)(pg_block(a.pool, page, kvh) + a.pool.v_off) + pg_v_at(HD, p & page_mask, 4 * hf);
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    const float y = (float)at[(32 * d + 8 * (v >> 2) + (v & 3)) * 8];
+                    if (!isfinite(y)) o[d][v] += y;
+                }
+        }
+    }
     l += __shfl_xor(l, 32);
     if (l != l) m = fmaxf(m, 0.0f);                    // a NaN score stays one
     if (!valid) return;

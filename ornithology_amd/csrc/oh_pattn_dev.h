@@ -65,6 +65,24 @@ OH_DEV void pg_codes(uint32_t lo, uint32_t hi, pg_h8 *o) {
 // before it is split into fp16 terms: top becomes 2^14 or more, below 2^15
 OH_DEV int pg_row_exp(float top) { return top > 0.0f && top < INFINITY ? 14 - max(ilogbf(top), -100) : 0; }
 
+// Values that are hidden from some row of a tile may be infinite or NaN
+// (another request's leavings behind the end, a prompt's later tokens), and a
+// weight of 0 times that is NaN: such tiles' values enter the products with 0
+// in those places, and where there was one (`odd`), it is added afterwards to
+// the rows that see it.
+template <bool H>
+OH_DEV bool pg_odd(uint32_t half) { return (half & (H ? 0x7c00u : 0x7f80u)) == (H ? 0x7c00u : 0x7f80u); }
+template <bool H>
+OH_DEV void pg_only_finite(uint4 *w, bool *odd) {
+    uint32_t *x = (uint32_t *)w;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const bool a = pg_odd<H>(x[i]), b = pg_odd<H>(x[i] >> 16);
+        *odd |= a || b;
+        x[i] = (a ? 0 : x[i] & 0xffffu) | (b ? 0 : x[i] & 0xffff0000u);
+    }
+}
+
 // ---- the batch ------------------------------------------------------------------
 // sequence s's rows and length, false (and reported) if they are not in range
 OH_DEV bool pg_seq(const oh_pattn &a, int s, int *row, int *n, int *len) {
