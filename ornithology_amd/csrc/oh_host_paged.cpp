@@ -80,9 +80,13 @@ int row_type(const char *who, const ornith_hip_paged *p, uint32_t type) {
 // A sequence's rows times the heads of a group decide: up to kFewRows they go to
 // the kernel for few rows; where all sequences have more, or could, to the one
 // for many.
-constexpr int kFewRows = 32, kManyRows = 128;
-int parts_of(int64_t most, int64_t blocks, int64_t want, int limit) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>(limit, std::min((most + 127) / 128, want / std::max<int64_t>(1, blocks))));
+constexpr int kFewRows = 32;
+// Parts of up to `most` positions for `units` pieces of work: as short as `least`,
+// and longer where that would make more than `blocks` blocks.
+int cut(int64_t most, int64_t units, int64_t blocks, int64_t least, int limit, int32_t *len) {
+    const int64_t n = std::max<int64_t>(1, std::min<int64_t>(limit, blocks / std::max<int64_t>(1, units)));
+    *len = (int32_t)std::min<int64_t>(INT32_MAX / 2, std::max(least, (most + n - 1) / n));
+    return (int)std::max<int64_t>(1, (most + *len - 1) / *len);
 }
 void plan(const ornith_hip_paged *p, const oh_pbatch &b, int nh, int n_group, oh_pattn *a) {
     const int nkv = p->pool.nkv, G = nh / nkv;
@@ -93,9 +97,14 @@ void plan(const ornith_hip_paged *p, const oh_pbatch &b, int nh, int n_group, oh
     a->few = widest <= kFewRows || (b.n_seq > 1 && b.n_rows < (int64_t)b.n_seq * b.max_new) ? kFewRows : 0;
     a->many = widest <= kFewRows ? -1 : a->few;
     a->gmany = all > kFewRows;
-    a->parts = a->few ? parts_of(most, (int64_t)b.n_seq * nkv, 2048, 64) : 1;
-    a->mparts = a->many >= 0 ? parts_of(most, (all / kManyRows + 1) * nkv, 768, 32) : 1;
-    a->gparts = !n_group ? 0 : a->gmany ? parts_of(most, (all / kManyRows + n_group) * nkv, 512, 64) : parts_of(most, n_group * nkv, 512, 64);
+    a->parts = a->mparts = 1;
+    a->gparts = 0;
+    a->least = a->mleast = a->gleast = 1;
+    // few rows: 128 positions are a tile for each wave of a block
+    if (a->few) a->parts = cut(most, (int64_t)b.n_seq * nkv, 8192, 128, 64, &a->least);
+    if (a->many >= 0) a->mparts = cut(most, (all / 256 + 1) * nkv, 512, 256, 32, &a->mleast);
+    if (n_group && a->gmany) a->gparts = cut(most, (all / 128 + n_group) * nkv, 256, 128, 64, &a->gleast);
+    else if (n_group) a->gparts = cut(most, (int64_t)n_group * nkv, 512, 128, 64, &a->gleast);
     a->sparts = std::max(a->parts, a->mparts);
 }
 uint64_t work_parts(const oh_pattn &a) {

@@ -28,7 +28,7 @@ pattn_few(oh_pattn a, int tiles_of_rows) {
     if (!pg_unit_at<PREFIX>(a, ui, &u)) return;
     const int G = a.G, F = u.n * G;
     if (rt * 16 >= F || (!PREFIX && F > a.few) || (PREFIX && !u.hi)) return;
-    const int parts = pg_parts(u.hi - u.lo, PREFIX ? a.gparts : a.parts);
+    const int parts = pg_parts(u.hi - u.lo, PREFIX ? a.gleast : a.least, PREFIX ? a.gparts : a.parts);
     if (c >= parts) return;
     const int64_t all = a.gparts + a.sparts, pc = PREFIX ? c : a.gparts + c;
     const bool direct = !PREFIX && parts == 1 && u.lo == 0;
@@ -72,120 +72,147 @@ pattn_few(oh_pattn a, int tiles_of_rows) {
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = (pg_f4){0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
+    // A tile's keys and values as they are in the pool, requested a tile (of this
+    // wave's) ahead: keys while the softmax and the values' products run, values
+    // from the end of the products on
+    constexpr int NU = HD / (Q8 ? 32 : 16);            // 16-byte units a lane and tile
+    uint4 kr[NU], vr[NU];
+    pg_f4 ks[2], vs[2], ks1[2], vs1[2];
     const int page_mask = (1 << a.pool.page_sh) - 1;
-    for (int t = t0 + wave; t < t1; t += 4) {
-        const int tb = 32 * t, page0 = u.pages[tb >> a.pool.page_sh];
-        const bool bad = page0 < 0 || page0 >= a.pool.n_pages;   // its positions are seen by no row
-        if (bad && lane == 0) pg_report(a.pool, OH_PF_PAGE);
-        const uint8_t *blk = pg_block(a.pool, bad ? 0 : page0, kvh);
-        const int slot = tb & page_mask;
-        const int vis = bad ? 0 : lim - tb;                      // positions of the tile below this are visible
-        const size_t tile = (size_t)(slot >> 5) * 32 * HD * (Q8 ? 1 : 2);
-        const uint8_t *kp = blk + tile, *vp = blk + a.pool.v_off + tile;
+    pg_list list = {u.pages, a.b.max_pages, 0, 0};
+    list.hold(32 * t0 >> a.pool.page_sh);
+    bool bad = false, odd = false;
+    const uint8_t *blk1;                               // of the next tile
+    bool there, there1;
+    auto tile_at = [&](int t) {
+        const int page = list.get(32 * t >> a.pool.page_sh);
+        there1 = page >= 0 && page < a.pool.n_pages;   // (if not, no row sees the tile)
+        bad |= !there1;
+        blk1 = pg_block(a.pool, there1 ? page : 0, kvh);
+    };
+    auto load_k = [&](int t) {
+        const uint8_t *at = blk1 + (size_t)((32 * t & page_mask) >> 5) * 32 * HD * (Q8 ? 1 : 2) + (g * 32 + n) * 16;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < NU / 2; i++) kr[h * NU / 2 + i] = ldg((const uint4 *)(at + i * 2048 + h * 256));
+        if (Q8) {
+            const float *sc = (const float *)(blk1 + a.pool.ks_off) + (32 * t & page_mask) + 4 * g;
+            const float *sv = (const float *)(blk1 + a.pool.vs_off) + (32 * t & page_mask) + 4 * g;
+#pragma unroll
+            for (int h = 0; h < 2; h++) { ks1[h] = ldg((const pg_f4 *)(sc + 16 * h)); vs1[h] = ldg((const pg_f4 *)(sv + 16 * h)); }
+        }
+    };
+    auto load_v = [&](int t, const uint8_t *b) {
+        const uint8_t *at = b + a.pool.v_off + (size_t)((32 * t & page_mask) >> 5) * 32 * HD * (Q8 ? 1 : 2) + g * HD * (Q8 ? 8 : 16) + n * 16;
+#pragma unroll
+        for (int i = 0; i < NU; i++) vr[i] = ldg((const uint4 *)(at + i * 256));
+    };
+    int t = t0 + wave;
+    if (t < t1) {
+        tile_at(t);
+        load_k(t);
+        load_v(t, blk1);
+    }
+    for (; t < t1; t += 4) {
+        there = there1;
+#pragma unroll
+        for (int h = 0; h < 2; h++) { ks[h] = ks1[h]; vs[h] = vs1[h]; }
+        const int tb = 32 * t, nt = t + 4 < t1 ? t + 4 : t;      // (at the end the same tile again, which is near)
+        const int vis = there ? lim - tb : 0;                    // positions of the tile below this are visible
         pg_f4 sc[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             sc[h] = (pg_f4){0.0f, 0.0f, 0.0f, 0.0f};
-            if (Q8) {
 #pragma unroll
-                for (int i = 0; i < NS / 2; i++) {
-                    const uint4 w = *(const uint4 *)(kp + ((4 * i + g) * 32 + 16 * h + n) * 16);
+            for (int i = 0; i < NU / 2; i++) {
+                const uint4 w = kr[h * NU / 2 + i];
+                if (Q8) {
                     kop k0, k1;
                     pg_codes(w.x, w.y, &k0);
                     pg_codes(w.z, w.w, &k1);
 #pragma unroll
-                    for (int k = NQ - 1; k >= 0; k--) {          // the small terms first
+                    for (int k = NQ - 1; k >= 0; k--) {          // the small term first
                         sc[h] = pg_mma16(k0, qf[k][2 * i], sc[h]);
                         sc[h] = pg_mma16(k1, qf[k][2 * i + 1], sc[h]);
                     }
+                } else {
+                    sc[h] = pg_mma16(__builtin_bit_cast(kop, w), qf[0][i], sc[h]);
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < NS; i++)
-                    sc[h] = pg_mma16(*(const kop *)(kp + ((4 * i + g) * 32 + 16 * h + n) * 16), qf[0][i], sc[h]);
             }
         }
+        tile_at(nt);
+        load_k(nt);
         float p[8];
         float mx = -INFINITY;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            pg_f4 ks = {1.0f, 1.0f, 1.0f, 1.0f};
-            if (Q8) ks = *(const pg_f4 *)(blk + a.pool.ks_off + 4 * (slot + 16 * h + 4 * g));
+        for (int h = 0; h < 2; h++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float x = Q8 ? sc[h][i] * ks[i] * unit : sc[h][i] * unit;
+                const float x = Q8 ? sc[h][i] * ks[h][i] * unit : sc[h][i] * unit;
                 p[4 * h + i] = 16 * h + 4 * g + i < vis ? x : -INFINITY;
                 mx = fmaxf(mx, p[4 * h + i]);
             }
-        }
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const float mn = fmaxf(m, mx);
-        const float alpha = mn == m ? 1.0f : pg_exp2(m - mn);
-        const float ref = mn == -INFINITY ? 0.0f : mn;           // (nothing seen, or keys of -inf)
-        m = mn;
-        l *= alpha;
+        if (__any(mn != m)) {
+            const float alpha = mn == m ? 1.0f : pg_exp2(m - mn);
+            l *= alpha;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            pg_f4 vs = {1.0f, 1.0f, 1.0f, 1.0f};
-            if (Q8) vs = *(const pg_f4 *)(blk + a.pool.vs_off + 4 * (slot + 16 * h + 4 * g));
+            for (int d = 0; d < ND; d++) o[d] *= alpha;
+            m = mn;
+        }
+        const float ref = mn == -INFINITY ? 0.0f : mn;           // (nothing seen, or keys of -inf)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const bool see = 16 * h + 4 * g + i < vis;
                 const float e = see ? pg_exp2(p[4 * h + i] - ref) : 0.0f;
                 l += e;
-                p[4 * h + i] = Q8 ? (see ? e * vs[i] : 0.0f) : e;
+                p[4 * h + i] = Q8 ? (see ? e * vs[h][i] : 0.0f) : e;
             }
-        }
         vop pf[NP];
         pg_split<NP>(p, pf);
+        if (!Q8 && __any(valid && vis < 32))
 #pragma unroll
-        for (int d = 0; d < ND; d++) o[d] *= alpha;
-        // Whole tiles hold finite values or ones that every row sees; where a
-        // row of the tile sees only a part, what it does not see (another
-        // request's leavings, a later token) may be infinite or NaN, and 0
-        // times that is NaN: such tiles go row by row, with those values zero
-        bool odd = false;
-        vop vf[ND];
+            for (int i = 0; i < NU; i++) pg_only_finite<ops::VH>(&vr[i], &odd);
 #pragma unroll
-        for (int d = 0; d < ND; d += 2) {
+        for (int i = 0; i < NU; i++) {
             if (Q8) {
-                const uint4 w = *(const uint4 *)(vp + (g * HD + 16 * d + 2 * n) * 8);
-                pg_codes(w.x, w.y, &vf[d]);
-                pg_codes(w.z, w.w, &vf[d + 1]);
-            } else {
-                vf[d] = *(const vop *)(vp + (g * HD + 16 * d + n) * 16);
-                vf[d + 1] = *(const vop *)(vp + (g * HD + 16 * (d + 1) + n) * 16);
-            }
-        }
-        if (!Q8 && __any(valid && vis < 32)) {
+                vop v0, v1;
+                pg_codes(vr[i].x, vr[i].y, &v0);
+                pg_codes(vr[i].z, vr[i].w, &v1);
 #pragma unroll
-            for (int d = 0; d < ND; d++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) odd |= !isfinite((float)vf[d][j]);
-            odd = __any(odd);
-        }
-        if (!odd) {
-#pragma unroll
-            for (int d = 0; d < ND; d++)
-#pragma unroll
-                for (int k = NP - 1; k >= 0; k--) o[d] = pg_mma16(vf[d], pf[k], o[d]);
-        } else {
-            for (int r = 0; r < 16; r++) {
-                const int v = __shfl(vis, r);                    // row r's
-                if (v <= 0) continue;
-#pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    vop x;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) x[j] = 16 * (j >> 2) + 4 * g + (j & 3) < v ? vf[d][j] : (typename ops::ve)0.0f;
-                    pg_f4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int k = NP - 1; k >= 0; k--) y = pg_mma16(x, pf[k], y);
-                    if (n == r) o[d] += y;
+                for (int k = NP - 1; k >= 0; k--) {
+                    o[2 * i] = pg_mma16(v0, pf[k], o[2 * i]);
+                    o[2 * i + 1] = pg_mma16(v1, pf[k], o[2 * i + 1]);
                 }
+            } else {
+#pragma unroll
+                for (int k = NP - 1; k >= 0; k--) o[i] = pg_mma16(__builtin_bit_cast(vop, vr[i]), pf[k], o[i]);
             }
         }
+        load_v(nt, blk1);
+    }
+    if (bad && lane == 0) pg_report(a.pool, OH_PF_PAGE);
+    if (!Q8 && __any(odd)) {
+        // the infinities and NaN of this wave's tiles, to the rows that see them:
+        // dims 16 d + 4 g + i
+        for (int t = t0 + wave; t < t1; t += 4)
+            for (int p = 32 * t; p < 32 * t + 32 && p < u.hi; p++) {
+                const int page = u.pages[p >> a.pool.page_sh];
+                if (p >= lim || __any(valid && lim - 32 * t < 32) == 0 || page < 0 || page >= a.pool.n_pages) continue;
+                const typename ops::ve *at = (const typename ops::ve *)(pg_block(a.pool, page, kvh) + a.pool.v_off) + pg_v_at(HD, p & page_mask, 4 * g);
+#pragma unroll
+                for (int d = 0; d < ND; d++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float y = (float)at[(16 * d + i) * 8];
+                        if (!isfinite(y)) o[d][i] += y;
+                    }
+            }
     }
     // the waves' results joined, 64 dims at a time
     l += __shfl_xor(l, 16);
@@ -238,45 +265,66 @@ pattn_few(oh_pattn a, int tiles_of_rows) {
     }
 }
 
-// Partial results joined: a wave takes one head of one row.
+// Partial results joined: a block takes one head of one row, each of its waves
+// every fourth part. A lane weighs a part of 64 at a time, so that the loads of
+// the parts' sums wait for no exponential.
 template <int RT, int HD>
 __global__ void __launch_bounds__(256)
 pattn_join(oh_pattn a) {
     typedef typename pg_elem<RT>::t row_t;
     constexpr int E = HD / 64;
+    typedef float fe __attribute__((ext_vector_type(E)));
+    __shared__ float ys[4][HD];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t item = (int64_t)blockIdx.x * 4 + wave;
-    const int r = (int)(item / a.nh), h = (int)(item % a.nh);
-    if (r >= a.b.n_rows) return;
+    const int r = (int)(blockIdx.x / a.nh), h = (int)(blockIdx.x % a.nh);
     const int s = pg_seq_of(a.pool, a.b, r);
     int row0, rows, len;
     if (s < 0 || !pg_seq(a, s, &row0, &rows, &len)) return;
     const int lo = pg_prefix_of(a, s);
-    const int parts = pg_parts(len - lo, rows * a.G <= a.few ? a.parts : a.mparts), gparts = lo ? pg_parts(lo, a.gparts) : 0;
+    const bool few = rows * a.G <= a.few;
+    const int parts = pg_parts(len - lo, few ? a.least : a.mleast, few ? a.parts : a.mparts), gparts = lo ? pg_parts(lo, a.gleast, a.gparts) : 0;
     if (parts == 1 && !gparts) return;                 // written already
-    const int64_t at = item * (a.gparts + a.sparts);
+    const int64_t at = (int64_t)blockIdx.x * (a.gparts + a.sparts);
     const int np = gparts + parts;
     // part c of np: the prefix's, then the sequence's own
+    auto where = [&](int c) { return at + (c < gparts ? c : a.gparts + c - gparts); };
     float M = -INFINITY;
-    for (int c = lane; c < np; c += 64) M = fmaxf(M, a.pml[at + (c < gparts ? c : a.gparts + c - gparts)].x);
+    for (int c = lane; c < np; c += 64) M = fmaxf(M, a.pml[where(c)].x);
 #pragma unroll
     for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
-    float L = 0.0f, y[E];
+    float L = 0.0f;
+    fe y;
 #pragma unroll
     for (int e = 0; e < E; e++) y[e] = 0.0f;
-    for (int c = 0; c < np; c++) {
-        const int64_t pc = at + (c < gparts ? c : a.gparts + c - gparts);
-        const float2 ml = a.pml[pc];
-        if (ml.x == -INFINITY) continue;               // nothing visible in it
-        const float w = pg_exp2(ml.x - M);
-        L = fmaf(ml.y, w, L);
+    for (int c0 = 0; c0 < np; c0 += 64) {
+        const int c = c0 + lane;
+        const float2 ml = c < np ? a.pml[where(c)] : make_float2(-INFINITY, 0.0f);
+        const float w = ml.x == -INFINITY ? 0.0f : pg_exp2(ml.x - M);      // (0: nothing visible in it)
+        if (w != 0.0f) L = fmaf(ml.y, w, L);
+        const int n = min(64, np - c0);
+        for (int i = wave; i < n; i += 16) {           // four requests together; lanes past the last part weigh 0
+            fe x[4];
 #pragma unroll
-        for (int e = 0; e < E; e++) y[e] = fmaf(a.po[pc * HD + lane * E + e], w, y[e]);
+            for (int j = 0; j < 4; j++) x[j] = *(const fe *)(a.po + where(min(c0 + i + 4 * j, np - 1)) * HD + lane * E);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float wi = i + 4 * j < n ? __shfl(w, (i + 4 * j) & 63) : 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; e++) y[e] = i + 4 * j < n ? fmaf(x[j][e], wi, y[e]) : y[e];
+            }
+        }
     }
-    const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
-    row_t *to = (row_t *)a.out.p + r * a.out.rs + h * a.out.hs + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; e++) to[e] = (row_t)(y[e] * inv);
+    for (int o = 32; o; o >>= 1) L += __shfl_xor(L, o);
+#pragma unroll
+    for (int e = 0; e < E; e++) ys[wave][lane * E + e] = y[e];
+    __syncthreads();
+    const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
+    row_t *to = (row_t *)a.out.p + r * a.out.rs + h * a.out.hs;
+    if ((int)threadIdx.x < HD) {
+        const int d = threadIdx.x;
+        to[d] = (row_t)(((ys[0][d] + ys[1][d]) + (ys[2][d] + ys[3][d])) * inv);
+    }
 }
 
 template <int RT, int CT, int HD>
@@ -294,7 +342,7 @@ hipError_t go_few(const oh_pattn *a, hipStream_t st) {
 }
 template <int RT, int CT, int HD>
 hipError_t go_join(const oh_pattn *a, hipStream_t st) {
-    const int64_t blocks = ((int64_t)a->b.n_rows * a->nh + 3) / 4;
+    const int64_t blocks = (int64_t)a->b.n_rows * a->nh;
     if (blocks > kMaxBlocks) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL((pattn_join<RT, HD>), dim3((unsigned)blocks), dim3(256), 0, st, *a);
     return hipGetLastError();

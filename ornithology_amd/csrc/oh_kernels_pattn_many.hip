@@ -30,7 +30,7 @@ template <int RT, int CT, int HD> struct many_cfg {
 
 template <int RT, int CT, int HD, bool PREFIX>
 __global__ void __launch_bounds__((64 * many_cfg<RT, CT, HD>::NW))
-pattn_many(oh_pattn a, int tiles_of_rows) {
+pattn_many(oh_pattn a) {
     typedef typename pg_elem<RT>::t row_t;
     typedef pg_ops<RT, CT> ops;
     typedef typename ops::kv kop;
@@ -44,21 +44,33 @@ pattn_many(oh_pattn a, int tiles_of_rows) {
     float *const lds_s = (float *)(lds + 4 * TILE);    // [2][keys' T, values' T]
     int *const lds_ok = (int *)(lds_s + 4 * T);        // [2][2]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hf = lane >> 5;
-    // long rows first: the last row tiles of a prompt see the most
-    const int ui = (int)blockIdx.x / tiles_of_rows, rt = tiles_of_rows - 1 - (int)blockIdx.x % tiles_of_rows;
-    const int kvh = blockIdx.y, c = blockIdx.z;
+    // The rows (times heads) are cut at multiples of TR and where units begin; a
+    // block takes one such piece. Unit i's first is piece i + 1 + (cuts up to
+    // it), so the unit of piece x is the last one whose first is not behind it,
+    // and a batch of one prompt among many single tokens has few idle blocks.
+    // Last rows first: they see the most.
+    const int piece = (int)(gridDim.x - 1 - blockIdx.x), kvh = blockIdx.y, c = blockIdx.z, G = a.G;
+    auto first = [&](int i) { return (int64_t)a.b.start[PREFIX ? min(max(a.gfirst[i], 0), a.b.n_seq) : i] * G; };
+    int ui = 0;
+    for (int hi = PREFIX ? a.n_group : a.b.n_seq; hi - ui > 1;) {
+        const int mid = (ui + hi) >> 1;
+        if (mid + 1 + first(mid) / TR <= piece) ui = mid; else hi = mid;
+    }
     pg_unit u;
     if (!pg_unit_at<PREFIX>(a, ui, &u)) return;
-    const int G = a.G, F = u.n * G;
-    if (rt * TR >= F || (!PREFIX && F <= a.many) || (PREFIX && !u.hi)) return;
-    const int parts = pg_parts(u.hi - u.lo, PREFIX ? a.gparts : a.mparts);
+    const int F = u.n * G;
+    const int64_t f0 = (int64_t)u.row * G, skip = piece - (ui + 1 + f0 / TR);            // cuts behind the unit's first row
+    const int64_t from = skip > 0 ? (f0 / TR + skip) * TR : f0, to = min((f0 / TR + skip + 1) * (int64_t)TR, f0 + F);
+    if (skip < 0 || from >= to || (!PREFIX && F <= a.many) || (PREFIX && !u.hi)) return;
+    const int parts = pg_parts(u.hi - u.lo, PREFIX ? a.gleast : a.mleast, PREFIX ? a.gparts : a.mparts);
     if (c >= parts) return;
     const int64_t pc = PREFIX ? c : a.gparts + c;
     const bool direct = !PREFIX && parts == 1 && u.lo == 0;
     int t0, t1;
     pg_part(u, c, parts, &t0, &t1);
-    const int f = rt * TR + wave * 32 + n, tok = u.row + f / G, head = kvh * G + f % G;
-    const bool valid = f < F;
+    const int64_t f = from + wave * 32 + n;
+    const int tok = (int)(f / G), head = kvh * G + (int)(f % G);
+    const bool valid = f < to;
     // what the lane's row sees of the part; the last position that some row of the
     // block sees, and the first that some row does not
     int lim = valid ? min(pg_unit_lim<PREFIX>(a, u, tok), 32 * t1) : 0;
@@ -416,21 +428,21 @@ pattn_many(oh_pattn a, int tiles_of_rows) {
 }
 
 template <int RT, int CT, int HD, bool PREFIX>
-hipError_t launch(const oh_pattn *a, int64_t rows, int units, int parts, hipStream_t st) {
+hipError_t launch(const oh_pattn *a, int units, int parts, hipStream_t st) {
     constexpr int NW = many_cfg<RT, CT, HD>::NW, lds = many_cfg<RT, CT, HD>::LDS;
-    const int64_t tiles = (rows * a->G + 32 * NW - 1) / (32 * NW);
-    if (tiles * units > kMaxBlocks / 2) return hipErrorInvalidConfiguration;
+    const int64_t pieces = (int64_t)a->b.n_rows * a->G / (32 * NW) + 1 + units;
+    if (pieces > kMaxBlocks / 2) return hipErrorInvalidConfiguration;
     const auto k = pattn_many<RT, CT, HD, PREFIX>;
     hipError_t e = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k, dim3((unsigned)(tiles * units), a->pool.nkv, parts), dim3(64 * NW), lds, st, *a, (int)tiles);
+    hipLaunchKernelGGL(k, dim3((unsigned)pieces, a->pool.nkv, parts), dim3(64 * NW), lds, st, *a);
     return hipGetLastError();
 }
 template <int RT, int CT, int HD>
 hipError_t go_many(const oh_pattn *a, hipStream_t st) {
     hipError_t e = hipSuccess;
-    if (a->n_group && a->gmany) e = launch<RT, CT, HD, true>(a, a->b.n_rows, a->n_group, a->gparts, st);
-    if (e == hipSuccess && a->many >= 0) e = launch<RT, CT, HD, false>(a, a->b.max_new, a->b.n_seq, a->mparts, st);
+    if (a->n_group && a->gmany) e = launch<RT, CT, HD, true>(a, a->n_group, a->gparts, st);
+    if (e == hipSuccess && a->many >= 0) e = launch<RT, CT, HD, false>(a, a->b.n_seq, a->mparts, st);
     return e;
 }
 

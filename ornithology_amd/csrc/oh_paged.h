@@ -71,6 +71,7 @@ struct oh_pattn {
     // and part c is at (r * nh + h) * (gparts + sparts) + c, the prefix's
     // first; sparts = max(parts, mparts)
     int32_t parts, mparts, gparts, sparts;
+    int32_t least, mleast, gleast;              // positions of a part, at least
     // sequences of up to `few` rows (times heads of a group) go to the one, of
     // more than `many` (-1: none) to the other; prefixes by gmany
     int32_t few, many, gmany;

@@ -71,16 +71,19 @@ OH_DEV int pg_row_exp(float top) { return top > 0.0f && top < INFINITY ? 14 - ma
 // in those places, and where there was one (`odd`), it is added afterwards to
 // the rows that see it.
 template <bool H>
-OH_DEV bool pg_odd(uint32_t half) { return (half & (H ? 0x7c00u : 0x7f80u)) == (H ? 0x7c00u : 0x7f80u); }
-template <bool H>
 OH_DEV void pg_only_finite(uint4 *w, bool *odd) {
-    uint32_t *x = (uint32_t *)w;
+    typedef unsigned short u2 __attribute__((ext_vector_type(2)));
+    constexpr uint32_t E = H ? 0x7c007c00u : 0x7f807f80u;                  // exponents of all ones
+    const u2 one = {1, 1}, zero = {0, 0};
+    uint32_t *x = (uint32_t *)w, all = ~0u;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const bool a = pg_odd<H>(x[i]), b = pg_odd<H>(x[i] >> 16);
-        *odd |= a || b;
-        x[i] = (a ? 0 : x[i] & 0xffffu) | (b ? 0 : x[i] & 0xffff0000u);
+        const u2 rest = __builtin_bit_cast(u2, (x[i] & E) ^ E);
+        const uint32_t keep = __builtin_bit_cast(uint32_t, zero - __builtin_elementwise_min(rest, one));
+        x[i] &= keep;
+        all &= keep;
     }
+    *odd |= all != ~0u;
 }
 
 // ---- the batch ------------------------------------------------------------------
@@ -166,11 +169,9 @@ struct pg_list {
     }
 };
 
-// parts of a stretch of n positions: at most `most`, of at least 4 tiles each
-// (a part's partial result is as large as two positions of a 16-bit pool)
-constexpr int kPartMin = 128;
-OH_DEV int pg_parts(int n, int most) {
-    const int p = (n + kPartMin - 1) / kPartMin;
+// parts of a stretch of n positions, each of at least `least` and at most `most` of them
+OH_DEV int pg_parts(int n, int least, int most) {
+    const int p = (n + least - 1) / least;
     return p < 1 ? 1 : p < most ? p : most;
 }
 // the 32-position tiles [t0, t1) of part c of a unit
