@@ -295,7 +295,8 @@ void ornith_hip_paged_free(ornith_hip_paged *p);
 int  ornith_hip_paged_faults(ornith_hip_paged *p, int32_t *faults);
 
 /* Store the batch's rows of keys and values at their positions. Keys are
- * normed first if k_norm is given (hd weights, x / sqrt(mean(x^2) + eps) * w), then
+ * normed first if k_norm is given (hd weights at a
+ * multiple of 16 bytes, x / sqrt(mean(x^2) + eps) * w), then
  * rotated; queries likewise (nh heads, q_norm), into q_out, which may be q
  * itself but not overlap it otherwise; q NULL: none. Rotation positions:
  * rope_pos[axis * rope_stride + row], or NULL: the cache position. */
@@ -314,8 +315,8 @@ int  ornith_hip_paged_read(const ornith_hip_paged *p, const ornith_hip_paged_bat
  * 0, nobody's are left as they were. out must not overlap q. The workspace
  * (16-byte aligned, contents undefined before and after) is at least what
  * ornith_hip_paged_workspace says for the batch's sizes. */
-int  ornith_hip_paged_workspace(const ornith_hip_paged *p, const ornith_hip_paged_batch *b, int nh, int n_group,
-                                uint64_t *bytes);
+int  ornith_hip_paged_workspace(const ornith_hip_paged *p, const ornith_hip_paged_batch *b, int nh, uint32_t type,
+                                int n_group, uint64_t *bytes);
 int  ornith_hip_paged_attend(const ornith_hip_paged *p, const ornith_hip_paged_batch *b, int nh, uint32_t type,
                              const ornith_hip_rows *q, const ornith_hip_rows *out, float scale, void *workspace,
                              uint64_t workspace_bytes, void *stream);

@@ -121,7 +121,7 @@ _SIGS = {
     "ornith_hip_paged_append": (C.c_int, [_vp, C.POINTER(_Batch), C.c_int, C.c_uint32, C.POINTER(_Rows), C.POINTER(_Rows),
                                           C.POINTER(_Rows), C.POINTER(_Rows), _vp, _vp, C.c_float, _vp, C.c_int64, _vp]),
     "ornith_hip_paged_read": (C.c_int, [_vp, C.POINTER(_Batch), C.c_uint32, C.POINTER(_Rows), C.POINTER(_Rows), _vp]),
-    "ornith_hip_paged_workspace": (C.c_int, [_vp, C.POINTER(_Batch), C.c_int, C.c_int, C.POINTER(C.c_uint64)]),
+    "ornith_hip_paged_workspace": (C.c_int, [_vp, C.POINTER(_Batch), C.c_int, C.c_uint32, C.c_int, C.POINTER(C.c_uint64)]),
     "ornith_hip_paged_attend": (C.c_int, [_vp, C.POINTER(_Batch), C.c_int, C.c_uint32, C.POINTER(_Rows), C.POINTER(_Rows),
                                           C.c_float, _vp, C.c_uint64, _vp]),
     "ornith_hip_paged_attend_prefix": (C.c_int, [_vp, C.POINTER(_Batch), C.c_int, _vp, _vp, C.c_int, C.c_uint32,
@@ -644,10 +644,11 @@ class PagedKV:
                "ornith_hip_paged_read")
         return k, v
 
-    def workspace(self, batch: PagedBatch, nh: int, n_group: int = 0) -> int:
-        """Bytes of workspace that attend (attend_prefix) needs for the batch's sizes."""
+    def workspace(self, batch: PagedBatch, nh: int, dtype, n_group: int = 0) -> int:
+        """Bytes of workspace that attend (attend_prefix) needs for the batch's sizes and rows of dtype."""
         n = C.c_uint64(0)
-        _check(lib().ornith_hip_paged_workspace(self.h, C.byref(batch.c), nh, n_group, C.byref(n)), "ornith_hip_paged_workspace")
+        _check(lib().ornith_hip_paged_workspace(self.h, C.byref(batch.c), nh, _row_type(dtype), n_group, C.byref(n)),
+               "ornith_hip_paged_workspace")
         return n.value
 
     def attend(self, batch: PagedBatch, q, *, scale: float | None = None, out=None, workspace=None):
@@ -675,7 +676,7 @@ class PagedKV:
         ro = self._rows("out", out, nh, batch.n_rows, q.dtype)
         n_group = 0 if first is None else length.numel()
         if workspace is None:
-            need = self.workspace(batch, nh, n_group)
+            need = self.workspace(batch, nh, q.dtype, n_group)
             workspace = t.empty(need, dtype=t.uint8, device=self.device) if need else None
         size = 0 if workspace is None else workspace.numel() * workspace.element_size()
         args = (nh, _row_type(q.dtype), C.byref(rq), C.byref(ro), self.hd ** -0.5 if scale is None else scale,

@@ -10,6 +10,7 @@ struct ornith_hip_paged {
     ornith_hip_ctx *ctx = nullptr;
     CtxRef ref;
     oh_pool pool;
+    int axes = 1;                               // of the rotation
     void *mem = nullptr, *aux = nullptr;        // the pages; the rotation's tables and the fault word
 };
 
@@ -102,8 +103,11 @@ void plan(const ornith_hip_paged *p, const oh_pbatch &b, int nh, int n_group, oh
     a->least = a->mleast = a->gleast = 1;
     // few rows: 128 positions are a tile for each wave of a block
     if (a->few) a->parts = cut(most, (int64_t)b.n_seq * nkv, 8192, 128, 64, &a->least);
-    if (a->many >= 0) a->mparts = cut(most, (all / 256 + 1) * nkv, 512, 256, 32, &a->mleast);
-    if (n_group && a->gmany) a->gparts = cut(most, (all / 128 + n_group) * nkv, 256, 128, 64, &a->gleast);
+    // many: a CU holds one block; two for each, so that the long ones' ends even out
+    int rows = 128;
+    (void)oh_pattn_many_rows(a, &rows);
+    if (a->many >= 0) a->mparts = cut(most, (all / rows + 1) * nkv, 512, 256, 32, &a->mleast);
+    if (n_group && a->gmany) a->gparts = cut(most, (all / rows + n_group) * nkv, 256, 128, 64, &a->gleast);
     else if (n_group) a->gparts = cut(most, (int64_t)n_group * nkv, 512, 128, 64, &a->gleast);
     a->sparts = std::max(a->parts, a->mparts);
 }
@@ -178,9 +182,10 @@ int pool_new(ornith_hip_ctx *ctx, const ornith_hip_paged_cfg *c, ornith_hip_page
         return ORNITH_HIP_ERR_FORMAT;
     }
     const int half = c->rope_dim / 2;
-    if (c->rope_axis)
-        for (int i = 0; i < half; i++)
-            if (c->rope_axis[i] > 3) { seterr("paged_new: axis %d of frequency %d (0 to 3)", c->rope_axis[i], i); return ORNITH_HIP_ERR_FORMAT; }
+    for (int i = 0; c->rope_axis && i < half; i++) {
+        if (c->rope_axis[i] > 3) { seterr("paged_new: axis %d of frequency %d (0 to 3)", c->rope_axis[i], i); return ORNITH_HIP_ERR_FORMAT; }
+        p->axes = std::max(p->axes, c->rope_axis[i] + 1);
+    }
     const uint32_t plane = (uint32_t)c->page_len * c->hd * type_bytes(c->type);
     o.nkv = c->nkv; o.hd = c->hd; o.type = (int32_t)c->type; o.n_pages = c->n_pages;
     while ((1 << o.page_sh) < c->page_len) o.page_sh++;
@@ -270,6 +275,8 @@ extern "C" int ornith_hip_paged_append(ornith_hip_paged *p, const ornith_hip_pag
     memset(&a, 0, sizeof a);
     CHK(batch_of(who, p, b, &a.b));
     CHK(row_type(who, p, type));
+    for (const float *w : {q_norm, k_norm})
+        if ((uintptr_t)w % 16) { seterr("%s: norm weights at %p, not a multiple of 16 bytes", who, (const void *)w); return ORNITH_HIP_ERR_UNSUPPORTED; }
     if (!(eps >= 0.0f)) { seterr("%s: eps %g", who, (double)eps); return ORNITH_HIP_ERR_FORMAT; }
     if (nothing(a.b)) return ORNITH_HIP_OK;
     CHK(placed(who, b));
@@ -283,7 +290,7 @@ extern "C" int ornith_hip_paged_append(ornith_hip_paged *p, const ornith_hip_pag
     }
     a.pool = p->pool;
     a.q_norm = q_norm; a.k_norm = k_norm; a.eps = eps;
-    a.pos = rope_pos; a.pos_stride = rope_stride;
+    a.pos = rope_pos; a.pos_stride = rope_stride; a.axes = p->axes;
     a.type = (int)type;
     OnDevice dev(p->ctx->device);
     HCHK(dev.e);
@@ -310,18 +317,20 @@ extern "C" int ornith_hip_paged_read(const ornith_hip_paged *p, const ornith_hip
     return ORNITH_HIP_OK;
 }
 
-extern "C" int ornith_hip_paged_workspace(const ornith_hip_paged *p, const ornith_hip_paged_batch *b, int nh, int n_group,
-                                          uint64_t *bytes) {
+extern "C" int ornith_hip_paged_workspace(const ornith_hip_paged *p, const ornith_hip_paged_batch *b, int nh, uint32_t type,
+                                          int n_group, uint64_t *bytes) {
     oh_pattn a;
     memset(&a, 0, sizeof a);
     if (!bytes) { seterr("paged_workspace: null result"); return ORNITH_HIP_ERR_FORMAT; }
     *bytes = 0;
     CHK(batch_of("paged_workspace", p, b, &a.b));
+    CHK(row_type("paged_workspace", p, type));
     CHK(heads("paged_workspace", p, nh));
     if (n_group < 0) { seterr("paged_workspace: %d groups", n_group); return ORNITH_HIP_ERR_FORMAT; }
     if (nothing(a.b)) return ORNITH_HIP_OK;
     CHK(placed("paged_workspace", b));
     a.pool = p->pool;
+    a.type = (int)type;
     plan(p, a.b, nh, n_group, &a);
     *bytes = work_bytes(a);
     return ORNITH_HIP_OK;

@@ -11,9 +11,9 @@ namespace {
 // (lane n = lane & 15 holds row n's scores of positions 4g..4g+3 and
 // 16+4g..+3, g = lane >> 4), the probabilities, and O^T += V^T P^T with the
 // probabilities where they are: the pool's value order matches.
-template <int RT, int CT, int HD, bool PREFIX>
+template <int RT, int CT, int HD>
 __global__ void __launch_bounds__(256)
-pattn_few(oh_pattn a, int tiles_of_rows) {
+pattn_few(oh_pattn a, int gblocks, int gtiles, int tiles) {
     typedef typename pg_elem<RT>::t row_t;
     typedef pg_ops<RT, CT> ops;
     typedef typename ops::kv kop;
@@ -23,31 +23,36 @@ pattn_few(oh_pattn a, int tiles_of_rows) {
     __shared__ float red[4][16][68];
     __shared__ float sm[4][16], sl[4][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    const int ui = (int)blockIdx.x / tiles_of_rows, rt = (int)blockIdx.x % tiles_of_rows, kvh = blockIdx.y, c = blockIdx.z;
+    // the first gblocks are the prefixes', gtiles of each group; then the sequences', tiles of each
+    const bool prefix = (int)blockIdx.x < gblocks;
+    const int bx = (int)blockIdx.x - (prefix ? 0 : gblocks), kvh = blockIdx.y, c = blockIdx.z;
+    const int ui = bx / (prefix ? gtiles : tiles), rt = bx % (prefix ? gtiles : tiles);
     pg_unit u;
-    if (!pg_unit_at<PREFIX>(a, ui, &u)) return;
+    if (!(prefix ? pg_unit_at<true>(a, ui, &u) : pg_unit_at<false>(a, ui, &u))) return;
     const int G = a.G, F = u.n * G;
-    if (rt * 16 >= F || (!PREFIX && F > a.few) || (PREFIX && !u.hi)) return;
-    const int parts = pg_parts(u.hi - u.lo, PREFIX ? a.gleast : a.least, PREFIX ? a.gparts : a.parts);
+    if (rt * 16 >= F || (!prefix && F > a.few) || (prefix && !u.hi)) return;
+    const int parts = pg_parts(u.hi - u.lo, prefix ? a.gleast : a.least, prefix ? a.gparts : a.parts);
     if (c >= parts) return;
-    const int64_t all = a.gparts + a.sparts, pc = PREFIX ? c : a.gparts + c;
-    const bool direct = !PREFIX && parts == 1 && u.lo == 0;
+    const int64_t all = a.gparts + a.sparts, pc = prefix ? c : a.gparts + c;
+    const bool direct = !prefix && parts == 1 && u.lo == 0;
     int t0, t1;
     pg_part(u, c, parts, &t0, &t1);
     // this lane's row
     const int f = rt * 16 + n, tok = u.row + f / G, head = kvh * G + f % G;
     const bool valid = f < F;
-    const int lim = valid ? pg_unit_lim<PREFIX>(a, u, tok) : 0;
-    const row_t *src = (const row_t *)a.q.p + tok * a.q.rs + head * a.q.hs;
+    const int lim = !valid ? 0 : prefix ? pg_unit_lim<true>(a, u, tok) : pg_unit_lim<false>(a, u, tok);
+    const row_t *src = (const row_t *)a.q.p + (valid ? tok * a.q.rs + head * a.q.hs : u.row * a.q.rs);
     kop qf[NQ][NS];
     float unit = a.scale;
     {
         float x[NS][8], top = 0.0f;
 #pragma unroll
+        for (int i = 0; i < NS; i++) pg_load<8>(src + (Q8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g), x[i]);
+#pragma unroll
         for (int i = 0; i < NS; i++)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                x[i][j] = valid ? (float)src[(Q8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g) + j] * a.sign : 0.0f;
+                x[i][j] = valid ? x[i][j] * a.sign : 0.0f;
                 top = fmaxf(top, fabsf(x[i][j]));
             }
         if (NQ > 1) {
@@ -255,9 +260,7 @@ pattn_few(oh_pattn a, int tiles_of_rows) {
             for (int i = 0; i < 4; i++)
                 y[i] = (red[0][wr][wd + i] + red[1][wr][wd + i] + red[2][wr][wd + i] + red[3][wr][wd + i]) * inv;
             if (direct) {
-                row_t *to = (row_t *)a.out.p + wtok * a.out.rs + whead * a.out.hs + 64 * q + wd;
-#pragma unroll
-                for (int i = 0; i < 4; i++) to[i] = (row_t)y[i];
+                pg_store<4>((row_t *)a.out.p + wtok * a.out.rs + whead * a.out.hs + 64 * q + wd, y);
             } else {
                 *(pg_f4 *)(a.po + (((int64_t)wtok * a.nh + whead) * all + pc) * HD + 64 * q + wd) = (pg_f4){y[0], y[1], y[2], y[3]};
             }
@@ -329,15 +332,12 @@ pattn_join(oh_pattn a) {
 
 template <int RT, int CT, int HD>
 hipError_t go_few(const oh_pattn *a, hipStream_t st) {
+    const bool groups = a->n_group && !a->gmany;
     const int64_t tiles = (std::min((int64_t)a->b.max_new * a->G, (int64_t)a->few) + 15) / 16;
-    if (tiles * a->b.n_seq > kMaxBlocks) return hipErrorInvalidConfiguration;
-    if (a->n_group && !a->gmany) {
-        const int64_t gtiles = ((int64_t)a->b.n_rows * a->G + 15) / 16;
-        if (gtiles * a->n_group > kMaxBlocks) return hipErrorInvalidConfiguration;
-        hipLaunchKernelGGL((pattn_few<RT, CT, HD, true>), dim3((unsigned)(gtiles * a->n_group), a->pool.nkv, a->gparts), dim3(256), 0, st, *a, (int)gtiles);
-    }
-    if (tiles)
-        hipLaunchKernelGGL((pattn_few<RT, CT, HD, false>), dim3((unsigned)(tiles * a->b.n_seq), a->pool.nkv, a->parts), dim3(256), 0, st, *a, (int)tiles);
+    const int64_t gtiles = groups ? ((int64_t)a->b.n_rows * a->G + 15) / 16 : 0, blocks = tiles * a->b.n_seq + gtiles * a->n_group;
+    if (blocks > kMaxBlocks) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((pattn_few<RT, CT, HD>), dim3((unsigned)blocks, a->pool.nkv, std::max(groups ? a->gparts : 1, a->parts)), dim3(256), 0, st,
+                       *a, (int)(gtiles * a->n_group), (int)gtiles, (int)tiles);
     return hipGetLastError();
 }
 template <int RT, int CT, int HD>

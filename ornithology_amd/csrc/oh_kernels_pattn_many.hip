@@ -94,12 +94,15 @@ pattn_many(oh_pattn a) {
     float unit = a.scale;                              // of the row's scores as they come out of the products
     {
         float x[NS][8], top = 0.0f;
-        const row_t *src = (const row_t *)a.q.p + tok * a.q.rs + head * a.q.hs + 8 * hf;
+        const row_t *src = (const row_t *)a.q.p + (valid ? tok * a.q.rs + head * a.q.hs : u.row * a.q.rs) + 8 * hf;
+#pragma unroll
+        for (int i = 0; i < NS; i++)
+            pg_load<8>(src + 16 * i, x[i]);
 #pragma unroll
         for (int i = 0; i < NS; i++)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                x[i][j] = valid ? (float)src[16 * i + j] * a.sign : 0.0f;
+                x[i][j] = valid ? x[i][j] * a.sign : 0.0f;
                 top = fmaxf(top, fabsf(x[i][j]));
             }
         if (NQ > 1) {
@@ -406,15 +409,14 @@ pattn_many(oh_pattn a) {
     if (direct) {
         const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
         row_t *to = (row_t *)a.out.p + tok * a.out.rs + head * a.out.hs + 4 * hf;
-        typedef row_t r4 __attribute__((ext_vector_type(4)));
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-                r4 y;
+                float y[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) y[i] = (row_t)(o[d][4 * q + i] * inv);
-                *(r4 *)(to + 32 * d + 8 * q) = y;
+                for (int i = 0; i < 4; i++) y[i] = o[d][4 * q + i] * inv;
+                pg_store<4>(to + 32 * d + 8 * q, y);
             }
     } else {
         const int64_t at = ((int64_t)tok * a.nh + head) * (a.gparts + a.sparts) + pc;
@@ -439,6 +441,11 @@ hipError_t launch(const oh_pattn *a, int units, int parts, hipStream_t st) {
     return hipGetLastError();
 }
 template <int RT, int CT, int HD>
+hipError_t go_rows(const oh_pattn *, int *rows) {
+    *rows = 32 * many_cfg<RT, CT, HD>::NW;
+    return hipSuccess;
+}
+template <int RT, int CT, int HD>
 hipError_t go_many(const oh_pattn *a, hipStream_t st) {
     hipError_t e = hipSuccess;
     if (a->n_group && a->gmany) e = launch<RT, CT, HD, true>(a, a->n_group, a->gparts, st);
@@ -448,4 +455,5 @@ hipError_t go_many(const oh_pattn *a, hipStream_t st) {
 
 } // namespace
 
+extern "C" hipError_t oh_pattn_many_rows(const oh_pattn *a, int *rows) { PG_TYPES(go_rows, a, rows) }
 extern "C" hipError_t oh_launch_pattn_many(const oh_pattn *a, hipStream_t st) { PG_TYPES(go_many, a, st) }

@@ -52,6 +52,7 @@ struct oh_pappend {
     float eps;
     const int32_t *pos;                         // null: the cache position on every axis
     int64_t pos_stride;                         // between axes
+    int32_t axes;                               // that the pool's frequencies name
     int32_t nh, type;                           // type of all rows
 };
 
@@ -87,5 +88,6 @@ hipError_t oh_launch_paged_append(const oh_pappend *a, hipStream_t st);
 hipError_t oh_launch_paged_read(const oh_pappend *a, hipStream_t st);
 hipError_t oh_launch_pattn_few(const oh_pattn *a, hipStream_t st);    // the sequences' (few) and the prefixes' (not gmany)
 hipError_t oh_launch_pattn_many(const oh_pattn *a, hipStream_t st);   // the sequences' (many) and the prefixes' (gmany)
+hipError_t oh_pattn_many_rows(const oh_pattn *a, int *rows);          // of a block, for a's types
 hipError_t oh_launch_pattn_join(const oh_pattn *a, hipStream_t st);
 }

@@ -47,6 +47,31 @@ OH_DEV int pg_seq_of(const oh_pool &p, const oh_pbatch &b, int r) {
     return lo;
 }
 
+// N (8 or 4) values of a row at p, which is a multiple of their size
+template <int N>
+OH_DEV void pg_load(const float *p, float (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        const pg_f4 w = ldg((const pg_f4 *)(p + i));
+        x[i] = w[0]; x[i + 1] = w[1]; x[i + 2] = w[2]; x[i + 3] = w[3];
+    }
+}
+template <int N, class T>
+OH_DEV void pg_load(const T *p, float (&x)[N]) {
+    typedef T v __attribute__((ext_vector_type(N)));
+    const v w = ldg((const v *)p);
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = (float)w[i];
+}
+template <int N, class T>
+OH_DEV void pg_store(T *p, const float (&x)[N]) {
+    typedef T v __attribute__((ext_vector_type(N)));
+    v w;
+#pragma unroll
+    for (int i = 0; i < N; i++) w[i] = (T)x[i];
+    *(v *)p = w;
+}
+
 // log2 of e
 constexpr float kLog2e = 1.44269504088896340736f;
 OH_DEV float pg_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
