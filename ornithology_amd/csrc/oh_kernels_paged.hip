@@ -241,50 +241,90 @@ paged_append(oh_pappend a, int qk_blocks, int heads, int span) {
     else append_v<RT, CT, HD>(a, blockIdx.x - qk_blocks, span);
 }
 
-// the stored rows of a batch, as values
+// The stored rows of a batch, as values. Keys as they are stored, 8 values a
+// lane; values of the rows that share a tile by way of LDS, which the tile's
+// units go through whole.
 template <int RT, int CT, int HD>
-__global__ void __launch_bounds__(256)
-paged_read(oh_pappend a) {
+OH_DEV void read_k(const oh_pappend &a, int block) {
     typedef typename pg_elem<RT>::t row_t;
     typedef typename pg_elem<CT>::t cache_t;
-    constexpr int E = HD / 64;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nkv = a.pool.nkv;
-    const int64_t item = (int64_t)blockIdx.x * 4 + wave;
-    const int r = (int)(item / (2 * nkv)), u = (int)(item % (2 * nkv));
-    if (r >= a.b.n_rows) return;
-    const int s = pg_seq_of(a.pool, a.b, r);
-    if (s < 0) return;
-    const int pos = a.b.len[s] - (a.b.start[s + 1] - r);
-    if (pos < 0) return;
-    const int pi = pos >> a.pool.page_sh;
-    if (pi >= a.b.max_pages) { if (lane == 0) pg_report(a.pool, OH_PF_BATCH); return; }
-    const int page = a.b.table[(size_t)s * a.b.max_pages + pi], slot = pos & ((1 << a.pool.page_sh) - 1);
-    if (page < 0 || page >= a.pool.n_pages) { if (lane == 0) pg_report(a.pool, OH_PF_PAGE); return; }
-    const bool isv = u >= nkv;
-    const int h = isv ? u - nkv : u;
-    const uint8_t *blk = pg_block(a.pool, page, h);
-    const cache_t *from = (const cache_t *)(blk + (isv ? a.pool.v_off : 0));
-    const float sc = CT == OH_PT_Q8 ? *(const float *)(blk + (isv ? a.pool.vs_off : a.pool.ks_off) + 4 * slot) : 1.0f;
-    const oh_prows &o = isv ? a.v : a.k;
-    row_t *to = (row_t *)o.p + r * o.rs + h * o.hs;
+    constexpr int L = head_lanes<HD>(), R = 256 / L;
+    const int tid = threadIdx.x, sub = tid % L, d0 = 8 * sub, head = block % a.pool.nkv, r = block / a.pool.nkv * R + tid / L;
+    place at;
+    if (!place_of(a.pool, a.b, r, &at)) return;
+    int slot;
+    const uint8_t *blk = slot_of(a.pool, a.b, at, head, &slot);
+    if (!blk) return;
+    float y[8];
+    pg_load<8>((const cache_t *)blk + pg_k_at<CT>(HD, slot, d0), y);
+    if (CT == OH_PT_Q8) {
+        const float sc = *(const float *)(blk + a.pool.ks_off + 4 * slot);
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        const int d = lane * E + e;
-        const float x = (float)from[isv ? pg_v_at(HD, slot, d) : pg_k_at<CT>(HD, slot, d)];
-        to[d] = (row_t)(CT == OH_PT_Q8 ? x * sc : x);
+        for (int j = 0; j < 8; j++) y[j] *= sc;
+    }
+    pg_store<8>((row_t *)a.k.p + r * a.k.rs + head * a.k.hs + d0, y);
+}
+template <int RT, int CT, int HD>
+OH_DEV void read_v(const oh_pappend &a, int block, int span) {
+    typedef typename pg_elem<RT>::t row_t;
+    typedef typename pg_elem<CT>::t cache_t;
+    typedef cache_t unit_t __attribute__((ext_vector_type(8)));
+    constexpr int L = head_lanes<HD>(), R = 256 / L;
+    __shared__ __align__(16) cache_t tile[32 * HD];
+    const int tid = threadIdx.x, sub = tid % L, d0 = 8 * sub, head = block % a.pool.nkv;
+    const int r1 = min(block / a.pool.nkv * span + span, a.b.n_rows);
+    auto at_unit = [](int u) { return u ^ ((u >> 3) & 7); };     // (as in append_v)
+    for (int r = block / a.pool.nkv * span; r < r1;) {
+        const int s = pg_seq_of(a.pool, a.b, r);
+        if (s < 0) { r++; continue; }
+        place at = {s, a.b.len[s] - (a.b.start[s + 1] - r)};
+        const int left = min(a.b.start[s + 1], r1) - r;
+        if (at.pos < 0) { r += at.pos <= -left ? left : -at.pos; continue; }
+        const int n = min(left, 32 - (at.pos & 31)), r0 = r;
+        r += n;
+        int slot;
+        const uint8_t *blk = slot_of(a.pool, a.b, at, head, &slot);
+        if (!blk) continue;
+        const cache_t *from = (const cache_t *)(blk + a.pool.v_off) + (slot >> 5) * 32 * HD;
+#pragma unroll
+        for (int k = 0; k < 4 * HD / 256; k++) {
+            const int u = tid + 256 * k;
+            *(unit_t *)(tile + at_unit(u) * 8) = *(const unit_t *)(from + u * 8);
+        }
+        __syncthreads();
+        for (int i = tid / L; i < n; i += R) {
+            const int sl = (slot & 31) + i;
+            const float sc = CT == OH_PT_Q8 ? *(const float *)(blk + a.pool.vs_off + 4 * (slot + i)) : 1.0f;
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float x = (float)tile[at_unit(((sl >> 2) & 3) * HD + d0 + j) * 8 + 4 * (sl >> 4) + (sl & 3)];
+                y[j] = CT == OH_PT_Q8 ? x * sc : x;
+            }
+            pg_store<8>((row_t *)a.v.p + (int64_t)(r0 + i) * a.v.rs + head * a.v.hs + d0, y);
+        }
+        __syncthreads();
     }
 }
+template <int RT, int CT, int HD>
+__global__ void __launch_bounds__(256)
+paged_read(oh_pappend a, int k_blocks, int span) {
+    if ((int)blockIdx.x < k_blocks) read_k<RT, CT, HD>(a, blockIdx.x);
+    else read_v<RT, CT, HD>(a, blockIdx.x - k_blocks, span);
+}
+
+// values go in stretches of 32 rows, but one by one where sequences bring few
+int span_of(const oh_pappend *a) { return a->b.n_rows >= (int64_t)8 * a->b.n_seq ? 32 : 1; }
 
 template <int RT, int CT, int HD>
 hipError_t append(const oh_pappend *a, hipStream_t st) {
     constexpr int R = 256 / head_lanes<HD>();
     // as many heads a block as leave 2048 blocks, so that few rows spread over the
-    // card and many rows form their sines and cosines once; the values in
-    // stretches of 32 rows, but one by one where sequences bring few
+    // card and many rows form their sines and cosines once
     const int64_t all = (a->q.p ? a->nh : 0) + a->pool.nkv, chunks = ((int64_t)a->b.n_rows + R - 1) / R;
     const int64_t heads = std::min(all, std::max<int64_t>(1, chunks * all / 2048));
     const int64_t qk = chunks * ((all + heads - 1) / heads);
-    const int span = a->b.n_rows >= (int64_t)8 * a->b.n_seq ? 32 : 1;
+    const int span = span_of(a);
     const int64_t v = ((int64_t)a->b.n_rows + span - 1) / span * a->pool.nkv;
     if (qk + v > kMaxBlocks) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL((paged_append<RT, CT, HD>), dim3((unsigned)(qk + v)), dim3(256), 0, st, *a, (int)qk, (int)heads, span);
@@ -292,9 +332,11 @@ hipError_t append(const oh_pappend *a, hipStream_t st) {
 }
 template <int RT, int CT, int HD>
 hipError_t read(const oh_pappend *a, hipStream_t st) {
-    const int64_t blocks = ((int64_t)a->b.n_rows * 2 * a->pool.nkv + 3) / 4;
-    if (blocks > kMaxBlocks) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((paged_read<RT, CT, HD>), dim3((unsigned)blocks), dim3(256), 0, st, *a);
+    constexpr int R = 256 / head_lanes<HD>();
+    const int span = span_of(a);
+    const int64_t k = ((int64_t)a->b.n_rows + R - 1) / R * a->pool.nkv, v = ((int64_t)a->b.n_rows + span - 1) / span * a->pool.nkv;
+    if (k + v > kMaxBlocks) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((paged_read<RT, CT, HD>), dim3((unsigned)(k + v)), dim3(256), 0, st, *a, (int)k, span);
     return hipGetLastError();
 }
 template <int RT, int CT>

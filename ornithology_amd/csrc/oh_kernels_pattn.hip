@@ -11,9 +11,51 @@ namespace {
 // (lane n = lane & 15 holds row n's scores of positions 4g..4g+3 and
 // 16+4g..+3, g = lane >> 4), the probabilities, and O^T += V^T P^T with the
 // probabilities where they are: the pool's value order matches.
+// Work is dealt out in items: (part of the positions, 16 rows, kv head) of a
+// prefix (`groups`: those of this kernel, before the sequences) or sequence. How
+// many a unit has is known on the device only, where the lengths are.
+struct few_item { int unit, rt, kvh, part; bool prefix; };
+OH_DEV int few_items(const oh_pattn &a, int groups, int x) {
+    pg_unit u;
+    const bool prefix = x < groups;
+    if (!(prefix ? pg_unit_at<true>(a, x, &u) : pg_unit_at<false>(a, x - groups, &u))) return 0;
+    const int F = u.n * a.G;
+    if (prefix ? !u.hi : F > a.few) return 0;
+    return pg_parts(u.hi - u.lo, prefix ? a.gleast : a.least, prefix ? a.gparts : a.parts) * ((F + 15) / 16) * a.pool.nkv;
+}
+// item i, false if there are fewer. The whole wave calls it; a lane counts one of 64 units.
+OH_DEV bool few_find(const oh_pattn &a, int groups, int i, few_item *o) {
+    const int lane = threadIdx.x & 63, n = groups + a.b.n_seq;
+    for (int x0 = 0, before = 0; x0 < n; x0 += 64) {
+        const int x = x0 + lane, mine = x < n ? few_items(a, groups, x) : 0;
+        int sum = mine;                                // of the units up to and with this lane's
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int y = __shfl_up(sum, d);
+            if (lane >= d) sum += y;
+        }
+        const uint64_t ends = __ballot(before + sum > i);
+        if (ends) {
+            const int l = __builtin_ctzll(ends);
+            const int left = i - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(mine, l));
+            pg_unit u;
+            o->prefix = x0 + l < groups;
+            o->unit = x0 + l - (o->prefix ? 0 : groups);
+            (void)(o->prefix ? pg_unit_at<true>(a, o->unit, &u) : pg_unit_at<false>(a, o->unit, &u));
+            const int tiles = (u.n * a.G + 15) / 16;
+            o->kvh = left % a.pool.nkv;
+            o->rt = left / a.pool.nkv % tiles;
+            o->part = left / a.pool.nkv / tiles;
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(sum, 63);
+    }
+    return false;
+}
+
 template <int RT, int CT, int HD>
 __global__ void __launch_bounds__(256)
-pattn_few(oh_pattn a, int gblocks, int gtiles, int tiles) {
+pattn_few(oh_pattn a, int groups) {
     typedef typename pg_elem<RT>::t row_t;
     typedef pg_ops<RT, CT> ops;
     typedef typename ops::kv kop;
@@ -23,16 +65,15 @@ pattn_few(oh_pattn a, int gblocks, int gtiles, int tiles) {
     __shared__ float red[4][16][68];
     __shared__ float sm[4][16], sl[4][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    // the first gblocks are the prefixes', gtiles of each group; then the sequences', tiles of each
-    const bool prefix = (int)blockIdx.x < gblocks;
-    const int bx = (int)blockIdx.x - (prefix ? 0 : gblocks), kvh = blockIdx.y, c = blockIdx.z;
-    const int ui = bx / (prefix ? gtiles : tiles), rt = bx % (prefix ? gtiles : tiles);
+    for (int item = blockIdx.x; ; item += gridDim.x) {
+    few_item it;
+    if (!few_find(a, groups, item, &it)) return;
+    const bool prefix = it.prefix;
+    const int rt = it.rt, kvh = it.kvh, c = it.part, G = a.G;
     pg_unit u;
-    if (!(prefix ? pg_unit_at<true>(a, ui, &u) : pg_unit_at<false>(a, ui, &u))) return;
-    const int G = a.G, F = u.n * G;
-    if (rt * 16 >= F || (!prefix && F > a.few) || (prefix && !u.hi)) return;
+    (void)(prefix ? pg_unit_at<true>(a, it.unit, &u) : pg_unit_at<false>(a, it.unit, &u));
+    const int F = u.n * G;
     const int parts = pg_parts(u.hi - u.lo, prefix ? a.gleast : a.least, prefix ? a.gparts : a.parts);
-    if (c >= parts) return;
     const int64_t all = a.gparts + a.sparts, pc = prefix ? c : a.gparts + c;
     const bool direct = !prefix && parts == 1 && u.lo == 0;
     int t0, t1;
@@ -266,6 +307,8 @@ pattn_few(oh_pattn a, int gblocks, int gtiles, int tiles) {
             }
         }
     }
+    __syncthreads();                                   // (the next item's results take the same place)
+    }
 }
 
 // Partial results joined: a block takes one head of one row, each of its waves
@@ -280,7 +323,7 @@ pattn_join(oh_pattn a) {
     __shared__ float ys[4][HD];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = (int)(blockIdx.x / a.nh), h = (int)(blockIdx.x % a.nh);
-    const int s = pg_seq_of(a.pool, a.b, r);
+    const int s = pg_seq_of_wave(a.pool, a.b, r);
     int row0, rows, len;
     if (s < 0 || !pg_seq(a, s, &row0, &rows, &len)) return;
     const int lo = pg_prefix_of(a, s);
@@ -332,12 +375,13 @@ pattn_join(oh_pattn a) {
 
 template <int RT, int CT, int HD>
 hipError_t go_few(const oh_pattn *a, hipStream_t st) {
-    const bool groups = a->n_group && !a->gmany;
-    const int64_t tiles = (std::min((int64_t)a->b.max_new * a->G, (int64_t)a->few) + 15) / 16;
-    const int64_t gtiles = groups ? ((int64_t)a->b.n_rows * a->G + 15) / 16 : 0, blocks = tiles * a->b.n_seq + gtiles * a->n_group;
-    if (blocks > kMaxBlocks) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((pattn_few<RT, CT, HD>), dim3((unsigned)blocks, a->pool.nkv, std::max(groups ? a->gparts : 1, a->parts)), dim3(256), 0, st,
-                       *a, (int)(gtiles * a->n_group), (int)gtiles, (int)tiles);
+    const int groups = a->gmany ? 0 : a->n_group;
+    // as many blocks as there can be items; where that is more than the card
+    // holds a few times over they take several
+    const int64_t tiles = (std::min((int64_t)a->b.max_new * a->G, (int64_t)a->few) + 15) / 16, gtiles = ((int64_t)a->b.n_rows * a->G + 15) / 16;
+    const int64_t items = (tiles * a->b.n_seq * a->parts + gtiles * groups * a->gparts) * a->pool.nkv;
+    const unsigned blocks = (unsigned)std::min<int64_t>(items, 1024);
+    hipLaunchKernelGGL((pattn_few<RT, CT, HD>), dim3(blocks), dim3(256), 0, st, *a, groups);
     return hipGetLastError();
 }
 template <int RT, int CT, int HD>

@@ -21,21 +21,22 @@ constexpr float kBehind = 8.0f;
 // Positions a step, waves a block, and whether the waves take turns: of the two
 // that share a SIMD one has its products while the other has its softmax. That
 // takes eight waves, so two sets of accumulators in a SIMD's registers.
-template <int RT, int CT, int HD> struct many_cfg {
-    static constexpr bool TURNS = RT != OH_PT_F32 && HD < 256 && !(CT == OH_PT_Q8 && HD == 64);
+template <int RT, int CT, int HD> constexpr bool can_turn() { return RT != OH_PT_F32 && HD < 256 && !(CT == OH_PT_Q8 && HD == 64); }
+template <int RT, int CT, int HD, bool TURN> struct many_cfg {
+    static constexpr bool TURNS = TURN;
     static constexpr int T = HD == 256 ? 32 : 64, NW = TURNS ? 8 : 4, H = T / 32;
     static constexpr int TILE = T * HD * 2;            // keys, or values, of a step in LDS, as 16-bit operands
     static constexpr int LDS = 4 * TILE + 2 * (8 * T + 16);   // two of each; scales and whether there is a page
 };
 
-template <int RT, int CT, int HD, bool PREFIX>
-__global__ void __launch_bounds__((64 * many_cfg<RT, CT, HD>::NW))
+template <int RT, int CT, int HD, bool PREFIX, bool TURN>
+__global__ void __launch_bounds__((64 * many_cfg<RT, CT, HD, TURN>::NW))
 pattn_many(oh_pattn a) {
     typedef typename pg_elem<RT>::t row_t;
     typedef pg_ops<RT, CT> ops;
     typedef typename ops::kv kop;
     typedef typename ops::vv vop;
-    typedef many_cfg<RT, CT, HD> cfg;
+    typedef many_cfg<RT, CT, HD, TURN> cfg;
     constexpr bool Q8 = CT == OH_PT_Q8;
     constexpr int NW = cfg::NW, T = cfg::T, H = cfg::H, TILE = cfg::TILE, NT = 64 * NW, TR = 32 * NW;
     constexpr int NQ = ops::NQ, NP = RT == OH_PT_F32 ? 3 : RT == OH_PT_F16 && Q8 ? 2 : 1, NS = HD / 16, ND = HD / 32;
@@ -51,11 +52,8 @@ pattn_many(oh_pattn a) {
     // Last rows first: they see the most.
     const int piece = (int)(gridDim.x - 1 - blockIdx.x), kvh = blockIdx.y, c = blockIdx.z, G = a.G;
     auto first = [&](int i) { return (int64_t)a.b.start[PREFIX ? min(max(a.gfirst[i], 0), a.b.n_seq) : i] * G; };
-    int ui = 0;
-    for (int hi = PREFIX ? a.n_group : a.b.n_seq; hi - ui > 1;) {
-        const int mid = (ui + hi) >> 1;
-        if (mid + 1 + first(mid) / TR <= piece) ui = mid; else hi = mid;
-    }
+    const int n_unit = PREFIX ? a.n_group : a.b.n_seq;
+    const int ui = max(pg_count(n_unit, [&](int i) { return i + 1 + first(i) / TR <= piece; }) - 1, 0);
     pg_unit u;
     if (!pg_unit_at<PREFIX>(a, ui, &u)) return;
     const int F = u.n * G;
@@ -429,27 +427,33 @@ pattn_many(oh_pattn a) {
     }
 }
 
-template <int RT, int CT, int HD, bool PREFIX>
+template <int RT, int CT, int HD, bool PREFIX, bool TURN>
 hipError_t launch(const oh_pattn *a, int units, int parts, hipStream_t st) {
-    constexpr int NW = many_cfg<RT, CT, HD>::NW, lds = many_cfg<RT, CT, HD>::LDS;
+    constexpr int NW = many_cfg<RT, CT, HD, TURN>::NW, lds = many_cfg<RT, CT, HD, TURN>::LDS;
     const int64_t pieces = (int64_t)a->b.n_rows * a->G / (32 * NW) + 1 + units;
     if (pieces > kMaxBlocks / 2) return hipErrorInvalidConfiguration;
-    const auto k = pattn_many<RT, CT, HD, PREFIX>;
+    const auto k = pattn_many<RT, CT, HD, PREFIX, TURN>;
     hipError_t e = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(k, dim3((unsigned)pieces, a->pool.nkv, parts), dim3(64 * NW), lds, st, *a);
     return hipGetLastError();
 }
+template <int RT, int CT, int HD, bool PREFIX>
+hipError_t with_turns(const oh_pattn *a, int rows, int units, int parts, hipStream_t st) {
+    if constexpr (can_turn<RT, CT, HD>())
+        if (rows == 256) return launch<RT, CT, HD, PREFIX, true>(a, units, parts, st);
+    return launch<RT, CT, HD, PREFIX, false>(a, units, parts, st);
+}
 template <int RT, int CT, int HD>
 hipError_t go_rows(const oh_pattn *, int *rows) {
-    *rows = 32 * many_cfg<RT, CT, HD>::NW;
+    *rows = can_turn<RT, CT, HD>() ? 256 : 128;
     return hipSuccess;
 }
 template <int RT, int CT, int HD>
 hipError_t go_many(const oh_pattn *a, hipStream_t st) {
     hipError_t e = hipSuccess;
-    if (a->n_group && a->gmany) e = launch<RT, CT, HD, true>(a, a->n_group, a->gparts, st);
-    if (e == hipSuccess && a->many >= 0) e = launch<RT, CT, HD, false>(a, a->b.n_seq, a->mparts, st);
+    if (a->n_group && a->gmany) e = with_turns<RT, CT, HD, true>(a, a->grows, a->n_group, a->gparts, st);
+    if (e == hipSuccess && a->many >= 0) e = with_turns<RT, CT, HD, false>(a, a->mrows, a->b.n_seq, a->mparts, st);
     return e;
 }
 

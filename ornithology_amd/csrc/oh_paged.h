@@ -76,6 +76,7 @@ struct oh_pattn {
     // sequences of up to `few` rows (times heads of a group) go to the one, of
     // more than `many` (-1: none) to the other; prefixes by gmany
     int32_t few, many, gmany;
+    int32_t mrows, grows;                       // rows of a block of the latter: 128, or up to oh_pattn_many_rows
     float *po;                                  // [..][hd], not divided by the sum
     float2 *pml;                                // [..] running maximum (log2) and sum
 };
@@ -88,6 +89,6 @@ hipError_t oh_launch_paged_append(const oh_pappend *a, hipStream_t st);
 hipError_t oh_launch_paged_read(const oh_pappend *a, hipStream_t st);
 hipError_t oh_launch_pattn_few(const oh_pattn *a, hipStream_t st);    // the sequences' (few) and the prefixes' (not gmany)
 hipError_t oh_launch_pattn_many(const oh_pattn *a, hipStream_t st);   // the sequences' (many) and the prefixes' (gmany)
-hipError_t oh_pattn_many_rows(const oh_pattn *a, int *rows);          // of a block, for a's types
+hipError_t oh_pattn_many_rows(const oh_pattn *a, int *rows);          // of a block, at most, for a's types
 hipError_t oh_launch_pattn_join(const oh_pattn *a, hipStream_t st);
 }

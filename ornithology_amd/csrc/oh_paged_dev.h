@@ -31,7 +31,29 @@ OH_DEV uint8_t *pg_block(const oh_pool &p, int page, int head) {
     return p.mem + ((size_t)page * p.nkv + head) * p.block;
 }
 
-// the sequence that row r belongs to, -1 (and reported) if `start` is no ascending list
+// How many of the indices [0, n) have p(i), for a p that holds up to some index
+// and not behind it: 64 at a time, one to a lane, so that a search costs a round
+// trip to memory and not one for each halving. The whole wave calls it.
+template <class P>
+OH_DEV int pg_count(int n, P p) {
+    int c = 0;
+    for (int i = 0; i < n; i += 64) {
+        const int at = i + (int)(threadIdx.x & 63);
+        const int k = (int)__popcll(__ballot(at < n && p(at)));
+        c += k;
+        if (k < 64) break;
+    }
+    return c;
+}
+// The sequence that row r (the same in the whole wave) belongs to, -1 (and
+// reported) if `start` is no ascending list
+OH_DEV int pg_seq_of_wave(const oh_pool &p, const oh_pbatch &b, int r) {
+    const int s = pg_count(b.n_seq, [&](int i) { return b.start[i + 1] <= r; });
+    if (s >= b.n_seq) return -1;                       // behind the last sequence: nobody's
+    if (r < b.start[s]) { pg_report(p, OH_PF_BATCH); return -1; }
+    return s;
+}
+// the same of a row of the lane's own
 OH_DEV int pg_seq_of(const oh_pool &p, const oh_pbatch &b, int r) {
     int lo = 0, hi = b.n_seq;                          // the last s with start[s] <= r
     while (hi - lo > 1) {

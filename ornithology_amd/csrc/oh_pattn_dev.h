@@ -105,7 +105,7 @@ OH_DEV int pg_shared(const oh_pattn &a, int i) {
     if (l < 0 || l > most) { pg_report(a.pool, OH_PF_BATCH); return 0; }
     return (l >> a.pool.page_sh) << a.pool.page_sh;
 }
-// the positions that sequence s leaves to its group's prefix
+// the positions that sequence s (of this lane) leaves to its group's prefix
 OH_DEV int pg_prefix_of(const oh_pattn &a, int s) {
     int lo = 0, hi = a.n_group;
     if (!hi) return 0;
