@@ -14,9 +14,9 @@ namespace {
 // Work is dealt out in items: (part of the positions, 16 rows, kv head) of a
 // prefix (`groups`: those of this kernel, before the sequences) or sequence. How
 // many a unit has is known on the device only, where the lengths are.
-struct few_item { int unit, rt, kvh, part; bool prefix; };
-OH_DEV int few_items(const oh_pattn &a, int groups, int x) {
-    pg_unit u;
+struct few_item { int rt, kvh, part; bool prefix; };
+OH_DEV int few_items(const oh_pattn &a, int groups, int x, pg_unit *o) {
+    pg_unit &u = *o;
     const bool prefix = x < groups;
     if (!(prefix ? pg_unit_at<true>(a, x, &u) : pg_unit_at<false>(a, x - groups, &u))) return 0;
     const int F = u.n * a.G;
@@ -24,10 +24,11 @@ OH_DEV int few_items(const oh_pattn &a, int groups, int x) {
     return pg_parts(u.hi - u.lo, prefix ? a.gleast : a.least, prefix ? a.gparts : a.parts) * ((F + 15) / 16) * a.pool.nkv;
 }
 // item i, false if there are fewer. The whole wave calls it; a lane counts one of 64 units.
-OH_DEV bool few_find(const oh_pattn &a, int groups, int i, few_item *o) {
+OH_DEV bool few_find(const oh_pattn &a, int groups, int i, few_item *o, pg_unit *u) {
     const int lane = threadIdx.x & 63, n = groups + a.b.n_seq;
     for (int x0 = 0, before = 0; x0 < n; x0 += 64) {
-        const int x = x0 + lane, mine = x < n ? few_items(a, groups, x) : 0;
+        pg_unit un = {0, 0, 0, 0, nullptr};
+        const int x = x0 + lane, mine = x < n ? few_items(a, groups, x, &un) : 0;
         int sum = mine;                                // of the units up to and with this lane's
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -38,11 +39,14 @@ OH_DEV bool few_find(const oh_pattn &a, int groups, int i, few_item *o) {
         if (ends) {
             const int l = __builtin_ctzll(ends);
             const int left = i - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(mine, l));
-            pg_unit u;
             o->prefix = x0 + l < groups;
-            o->unit = x0 + l - (o->prefix ? 0 : groups);
-            (void)(o->prefix ? pg_unit_at<true>(a, o->unit, &u) : pg_unit_at<false>(a, o->unit, &u));
-            const int tiles = (u.n * a.G + 15) / 16;
+            u->row = __builtin_amdgcn_readlane(un.row, l);
+            u->n = __builtin_amdgcn_readlane(un.n, l);
+            u->lo = __builtin_amdgcn_readlane(un.lo, l);
+            u->hi = __builtin_amdgcn_readlane(un.hi, l);
+            const int64_t at = (int64_t)(un.pages - a.b.table);
+            u->pages = a.b.table + ((int64_t)__builtin_amdgcn_readlane((int)(at >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)at, l));
+            const int tiles = (u->n * a.G + 15) / 16;
             o->kvh = left % a.pool.nkv;
             o->rt = left / a.pool.nkv % tiles;
             o->part = left / a.pool.nkv / tiles;
@@ -67,11 +71,10 @@ pattn_few(oh_pattn a, int groups) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
     for (int item = blockIdx.x; ; item += gridDim.x) {
     few_item it;
-    if (!few_find(a, groups, item, &it)) return;
+    pg_unit u;
+    if (!few_find(a, groups, item, &it, &u)) return;
     const bool prefix = it.prefix;
     const int rt = it.rt, kvh = it.kvh, c = it.part, G = a.G;
-    pg_unit u;
-    (void)(prefix ? pg_unit_at<true>(a, it.unit, &u) : pg_unit_at<false>(a, it.unit, &u));
     const int F = u.n * G;
     const int parts = pg_parts(u.hi - u.lo, prefix ? a.gleast : a.least, prefix ? a.gparts : a.parts);
     const int64_t all = a.gparts + a.sparts, pc = prefix ? c : a.gparts + c;
@@ -82,38 +85,13 @@ pattn_few(oh_pattn a, int groups) {
     const int f = rt * 16 + n, tok = u.row + f / G, head = kvh * G + f % G;
     const bool valid = f < F;
     const int lim = !valid ? 0 : prefix ? pg_unit_lim<true>(a, u, tok) : pg_unit_lim<false>(a, u, tok);
+    // requests first: the page list, the queries, the first tile
+    pg_list list = {u.pages, a.b.max_pages, 0, 0};
+    list.hold(32 * t0 >> a.pool.page_sh);
     const row_t *src = (const row_t *)a.q.p + (valid ? tok * a.q.rs + head * a.q.hs : u.row * a.q.rs);
-    kop qf[NQ][NS];
-    float unit = a.scale;
-    {
-        float x[NS][8], top = 0.0f;
+    float x[NS][8], top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NS; i++) pg_load<8>(src + (Q8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g), x[i]);
-#pragma unroll
-        for (int i = 0; i < NS; i++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                x[i][j] = valid ? x[i][j] * a.sign : 0.0f;
-                top = fmaxf(top, fabsf(x[i][j]));
-            }
-        if (NQ > 1) {
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const int e = pg_row_exp(top);
-            unit = ldexpf(unit, -e);
-#pragma unroll
-            for (int i = 0; i < NS; i++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[i][j] = ldexpf(x[i][j], e);
-        }
-#pragma unroll
-        for (int i = 0; i < NS; i++) {
-            kop t[NQ];
-            pg_split<NQ>(x[i], t);
-#pragma unroll
-            for (int k = 0; k < NQ; k++) qf[k][i] = t[k];
-        }
-    }
+    for (int i = 0; i < NS; i++) pg_load<8>(src + (Q8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g), x[i]);
     pg_f4 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = (pg_f4){0.0f, 0.0f, 0.0f, 0.0f};
@@ -125,8 +103,6 @@ pattn_few(oh_pattn a, int groups) {
     uint4 kr[NU], vr[NU];
     pg_f4 ks[2], vs[2], ks1[2], vs1[2];
     const int page_mask = (1 << a.pool.page_sh) - 1;
-    pg_list list = {u.pages, a.b.max_pages, 0, 0};
-    list.hold(32 * t0 >> a.pool.page_sh);
     bool bad = false, odd = false;
     const uint8_t *blk1;                               // of the next tile
     bool there, there1;
@@ -159,6 +135,34 @@ pattn_few(oh_pattn a, int groups) {
         tile_at(t);
         load_k(t);
         load_v(t, blk1);
+    }
+    kop qf[NQ][NS];
+    float unit = a.scale;
+    {
+#pragma unroll
+        for (int i = 0; i < NS; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                x[i][j] = valid ? x[i][j] * a.sign : 0.0f;
+                top = fmaxf(top, fabsf(x[i][j]));
+            }
+        if (NQ > 1) {
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const int e = pg_row_exp(top);
+            unit = ldexpf(unit, -e);
+#pragma unroll
+            for (int i = 0; i < NS; i++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[i][j] = ldexpf(x[i][j], e);
+        }
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+            kop t[NQ];
+            pg_split<NQ>(x[i], t);
+#pragma unroll
+            for (int k = 0; k < NQ; k++) qf[k][i] = t[k];
+        }
     }
     for (; t < t1; t += 4) {
         there = there1;
@@ -311,8 +315,8 @@ pattn_few(oh_pattn a, int groups) {
     }
 }
 
-// Partial results joined: a block takes one head of one row, each of its waves
-// every fourth part. A lane weighs a part of 64 at a time, so that the loads of
+// Partial results joined: a block takes one row and some of its heads, each of
+// its waves every fourth part. A lane weighs a part of 64 at a time, so that the loads of
 // the parts' sums wait for no exponential.
 template <int RT, int HD>
 __global__ void __launch_bounds__(256)
@@ -322,7 +326,7 @@ pattn_join(oh_pattn a) {
     typedef float fe __attribute__((ext_vector_type(E)));
     __shared__ float ys[4][HD];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int r = (int)(blockIdx.x / a.nh), h = (int)(blockIdx.x % a.nh);
+    const int r = blockIdx.x;
     const int s = pg_seq_of_wave(a.pool, a.b, r);
     int row0, rows, len;
     if (s < 0 || !pg_seq(a, s, &row0, &rows, &len)) return;
@@ -330,8 +334,9 @@ pattn_join(oh_pattn a) {
     const bool few = rows * a.G <= a.few;
     const int parts = pg_parts(len - lo, few ? a.least : a.mleast, few ? a.parts : a.mparts), gparts = lo ? pg_parts(lo, a.gleast, a.gparts) : 0;
     if (parts == 1 && !gparts) return;                 // written already
-    const int64_t at = (int64_t)blockIdx.x * (a.gparts + a.sparts);
     const int np = gparts + parts;
+    for (int h = blockIdx.y; h < a.nh; h += gridDim.y) {
+    const int64_t at = ((int64_t)r * a.nh + h) * (a.gparts + a.sparts);
     // part c of np: the prefix's, then the sequence's own
     auto where = [&](int c) { return at + (c < gparts ? c : a.gparts + c - gparts); };
     float M = -INFINITY;
@@ -371,6 +376,8 @@ pattn_join(oh_pattn a) {
         const int d = threadIdx.x;
         to[d] = (row_t)(((ys[0][d] + ys[1][d]) + (ys[2][d] + ys[3][d])) * inv);
     }
+    __syncthreads();                                   // (ys is the next head's)
+    }
 }
 
 template <int RT, int CT, int HD>
@@ -386,9 +393,10 @@ hipError_t go_few(const oh_pattn *a, hipStream_t st) {
 }
 template <int RT, int CT, int HD>
 hipError_t go_join(const oh_pattn *a, hipStream_t st) {
-    const int64_t blocks = (int64_t)a->b.n_rows * a->nh;
-    if (blocks > kMaxBlocks) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((pattn_join<RT, HD>), dim3((unsigned)blocks), dim3(256), 0, st, *a);
+    // (a prompt's rows have mostly nothing to join: few blocks for them)
+    const int64_t heads = std::min<int64_t>(a->nh, std::max<int64_t>(1, 4096 / a->b.n_rows));
+    if (a->b.n_rows > kMaxBlocks) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((pattn_join<RT, HD>), dim3((unsigned)a->b.n_rows, (unsigned)heads), dim3(256), 0, st, *a);
     return hipGetLastError();
 }
 

@@ -21,6 +21,9 @@ constexpr float kBehind = 8.0f;
 // Positions a step, waves a block, and whether the waves take turns: of the two
 // that share a SIMD one has its products while the other has its softmax. That
 // takes eight waves, so two sets of accumulators in a SIMD's registers.
+// the largest power of two up to 8 that divides n
+__host__ __device__ inline int gcd8(int n) { return n % 8 == 0 ? 8 : n % 4 == 0 ? 4 : n % 2 == 0 ? 2 : 1; }
+
 template <int RT, int CT, int HD> constexpr bool can_turn() { return RT != OH_PT_F32 && HD < 256 && !(CT == OH_PT_Q8 && HD == 64); }
 template <int RT, int CT, int HD, bool TURN> struct many_cfg {
     static constexpr bool TURNS = TURN;
@@ -31,7 +34,7 @@ template <int RT, int CT, int HD, bool TURN> struct many_cfg {
 
 template <int RT, int CT, int HD, bool PREFIX, bool TURN>
 __global__ void __launch_bounds__((64 * many_cfg<RT, CT, HD, TURN>::NW))
-pattn_many(oh_pattn a) {
+pattn_many(oh_pattn a, int pieces) {
     typedef typename pg_elem<RT>::t row_t;
     typedef pg_ops<RT, CT> ops;
     typedef typename ops::kv kop;
@@ -50,7 +53,11 @@ pattn_many(oh_pattn a) {
     // it), so the unit of piece x is the last one whose first is not behind it,
     // and a batch of one prompt among many single tokens has few idle blocks.
     // Last rows first: they see the most.
-    const int piece = (int)(gridDim.x - 1 - blockIdx.x), kvh = blockIdx.y, c = blockIdx.z, G = a.G;
+    // Blocks go to the eight XCDs in turn, each with an L2 of its own: the pieces of
+    // a head are dealt to those XCDs that hold no other head than they must.
+    const int xcd = blockIdx.x % 8, g8 = gcd8(a.pool.nkv), mine = (int)(blockIdx.x / 8) * (8 / g8) + xcd / g8;
+    const int kvh = mine / pieces * g8 + xcd % g8, piece = pieces - 1 - mine % pieces, c = blockIdx.y, G = a.G;
+    if (kvh >= a.pool.nkv) return;
     auto first = [&](int i) { return (int64_t)a.b.start[PREFIX ? min(max(a.gfirst[i], 0), a.b.n_seq) : i] * G; };
     const int n_unit = PREFIX ? a.n_group : a.b.n_seq;
     const int ui = max(pg_count(n_unit, [&](int i) { return i + 1 + first(i) / TR <= piece; }) - 1, 0);
@@ -90,35 +97,6 @@ pattn_many(oh_pattn a) {
 
     kop qf[NQ][NS];
     float unit = a.scale;                              // of the row's scores as they come out of the products
-    {
-        float x[NS][8], top = 0.0f;
-        const row_t *src = (const row_t *)a.q.p + (valid ? tok * a.q.rs + head * a.q.hs : u.row * a.q.rs) + 8 * hf;
-#pragma unroll
-        for (int i = 0; i < NS; i++)
-            pg_load<8>(src + 16 * i, x[i]);
-#pragma unroll
-        for (int i = 0; i < NS; i++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                x[i][j] = valid ? x[i][j] * a.sign : 0.0f;
-                top = fmaxf(top, fabsf(x[i][j]));
-            }
-        if (NQ > 1) {
-            const int e = pg_row_exp(fmaxf(top, __shfl_xor(top, 32)));
-            unit = ldexpf(unit, -e);
-#pragma unroll
-            for (int i = 0; i < NS; i++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[i][j] = ldexpf(x[i][j], e);
-        }
-#pragma unroll
-        for (int i = 0; i < NS; i++) {
-            kop t[NQ];
-            pg_split<NQ>(x[i], t);
-#pragma unroll
-            for (int k = 0; k < NQ; k++) qf[k][i] = t[k];
-        }
-    }
     pg_f16 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++)
@@ -330,6 +308,35 @@ pattn_many(oh_pattn a) {
     // nothing: no branch splits the loops' registers.
     fetch(lk, p0, 0, kr, true);
     if (!cfg::TURNS) fetch(lv, p0, a.pool.v_off, vr);
+    {
+        float x[NS][8], top = 0.0f;
+        const row_t *src = (const row_t *)a.q.p + (valid ? tok * a.q.rs + head * a.q.hs : u.row * a.q.rs) + 8 * hf;
+#pragma unroll
+        for (int i = 0; i < NS; i++)
+            pg_load<8>(src + 16 * i, x[i]);
+#pragma unroll
+        for (int i = 0; i < NS; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                x[i][j] = valid ? x[i][j] * a.sign : 0.0f;
+                top = fmaxf(top, fabsf(x[i][j]));
+            }
+        if (NQ > 1) {
+            const int e = pg_row_exp(fmaxf(top, __shfl_xor(top, 32)));
+            unit = ldexpf(unit, -e);
+#pragma unroll
+            for (int i = 0; i < NS; i++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[i][j] = ldexpf(x[i][j], e);
+        }
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+            kop t[NQ];
+            pg_split<NQ>(x[i], t);
+#pragma unroll
+            for (int k = 0; k < NQ; k++) qf[k][i] = t[k];
+        }
+    }
     stage_k(0);
     if (!cfg::TURNS) stage_v(0);
     __syncthreads();
@@ -431,11 +438,13 @@ template <int RT, int CT, int HD, bool PREFIX, bool TURN>
 hipError_t launch(const oh_pattn *a, int units, int parts, hipStream_t st) {
     constexpr int NW = many_cfg<RT, CT, HD, TURN>::NW, lds = many_cfg<RT, CT, HD, TURN>::LDS;
     const int64_t pieces = (int64_t)a->b.n_rows * a->G / (32 * NW) + 1 + units;
-    if (pieces > kMaxBlocks / 2) return hipErrorInvalidConfiguration;
+    const int g8 = gcd8(a->pool.nkv);                  // heads' residues, each with 8 / g8 XCDs
+    const int64_t blocks = 8 * ((pieces * (a->pool.nkv / g8) + 8 / g8 - 1) / (8 / g8));
+    if (blocks > kMaxBlocks / 2) return hipErrorInvalidConfiguration;
     const auto k = pattn_many<RT, CT, HD, PREFIX, TURN>;
     hipError_t e = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k, dim3((unsigned)pieces, a->pool.nkv, parts), dim3(64 * NW), lds, st, *a);
+    hipLaunchKernelGGL(k, dim3((unsigned)blocks, parts), dim3(64 * NW), lds, st, *a, (int)pieces);
     return hipGetLastError();
 }
 template <int RT, int CT, int HD, bool PREFIX>
