@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import weakref
 from pathlib import Path
 
 import numpy as np
@@ -519,23 +520,26 @@ class Session:
 
 # ---- paged key/value pool: device buffers, as torch tensors -----------------------
 
-def _torch():
-    """torch, for the calls on device tensors. It brings a HIP runtime of its own,
-    which the library shares if torch is imported before its first use."""
-    import torch
-    return torch
-
-
+_t = None                                    # torch, once a call on device tensors has asked for it
 _row_types = {}
 
 
+def _torch():
+    """torch, for the calls on device tensors. It brings a HIP runtime of its own,
+    which the library shares if torch is imported before its first use."""
+    global _t
+    if _t is None:
+        import torch
+        _row_types.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+        _t = torch
+    return _t
+
+
 def _row_type(dtype) -> int:
-    if not _row_types:
-        t = _torch()
-        _row_types.update({t.float32: F32, t.float16: F16, t.bfloat16: BF16})
-    if dtype not in _row_types:
+    k = _row_types.get(dtype)
+    if k is None:
         raise ValueError(f"rows of {dtype}: float32, float16 or bfloat16")
-    return _row_types[dtype]
+    return k
 
 
 class PagedBatch:
@@ -553,9 +557,11 @@ class PagedBatch:
             if x.device != kv_len.device:
                 raise ValueError("PagedBatch: lists on different devices")
         self.seq_start, self.kv_len, self.pages, self.n_rows = seq_start, kv_len, pages, int(n_rows)
-        self.device = kv_len.device
+        self.device, self.index = kv_len.device, kv_len.get_device()
         self.c = _Batch(seq_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr(), n, self.n_rows, pages.shape[1],
                         self.n_rows if max_new is None else int(max_new))
+        self.ref = C.byref(self.c)
+        self.needs = weakref.WeakKeyDictionary()   # workspace bytes, by pool and (heads, type, groups)
 
 
 class PagedKV:
@@ -579,7 +585,7 @@ class PagedKV:
         self.ctx, self.h = ctx, h
         self.n_pages, self.nkv, self.hd, self.page_len, self.type = n_pages, nkv, hd, page_len, type
         self.axes = 1 + (int(axis.max()) if axis is not None and axis.size else 0)
-        self.device = t.device("cuda", ctx.device)
+        self.device, self.index = t.device("cuda", ctx.device), ctx.device
         probe = t.empty(1, device=self.device)
         if lib().hipPointerGetAttributes(C.create_string_buffer(256), C.c_void_p(probe.data_ptr())) != 0:
             self.free()
@@ -587,67 +593,62 @@ class PagedKV:
                                "first use of ornithology_amd")
 
     def _rows(self, name, x, heads, n_rows, dtype):
-        if x.dtype != dtype or x.dim() != 3 or x.shape[1] != heads or x.shape[2] != self.hd or x.shape[0] < n_rows:
-            raise ValueError(f"{name} is {x.dtype} {tuple(x.shape)}, not {dtype} [{n_rows}, {heads}, {self.hd}]")
-        if x.device != self.device or x.stride(2) != 1:
+        shape, (s0, s1, s2) = x.shape, x.stride() if x.dim() == 3 else (0, 0, 0)
+        if x.dtype != dtype or len(shape) != 3 or shape[1] != heads or shape[2] != self.hd or shape[0] < n_rows:
+            raise ValueError(f"{name} is {x.dtype} {tuple(shape)}, not {dtype} [{n_rows}, {heads}, {self.hd}]")
+        if x.get_device() != self.index or s2 != 1:
             raise ValueError(f"{name}: on {x.device} (the pool on {self.device}) with strides {x.stride()}; heads are contiguous")
-        if x.requires_grad and _torch().is_grad_enabled():
+        if x.requires_grad and _t.is_grad_enabled():
             raise ValueError(f"{name} requires a gradient: these operators have no backward pass")
-        return _Rows(x.data_ptr(), x.stride(0) if x.shape[0] > 1 else 0, x.stride(1) if heads > 1 else 0)
+        return _Rows(x.data_ptr(), s0 if shape[0] > 1 else 0, s1 if heads > 1 else 0)
 
     def _begin(self, batch):
         if self.h is None:
             raise ValueError("the pool is freed")
-        if batch.device != self.device:
+        if batch.index != self.index:
             raise ValueError(f"the batch is on {batch.device}, the pool on {self.device}")
-        return C.c_void_p(_torch().cuda.current_stream(self.device).cuda_stream)
+        return _t.cuda.current_stream(self.index).cuda_stream
 
     def _vector(self, name, x):
         if x is None:
             return None
-        t = _torch()
-        if x.dtype != t.float32 or x.numel() != self.hd or not x.is_contiguous() or x.device != self.device:
+        if x.dtype != _t.float32 or x.numel() != self.hd or not x.is_contiguous() or x.get_device() != self.index:
             raise ValueError(f"{name}: {self.hd} contiguous float32 weights on {self.device}")
-        return C.c_void_p(x.data_ptr())
+        return x.data_ptr()
 
     def append(self, batch: PagedBatch, k, v, *, q=None, q_out=None, q_norm=None, k_norm=None, eps: float = 1e-6, rope_pos=None):
         """Store the batch's rows of keys (normed, rotated) and values, and
         return q normed and rotated (in q_out, a new tensor by default).
         rope_pos: int32 [axes, n_rows], default: the cache positions."""
-        t, st = _torch(), self._begin(batch)
-        n = batch.n_rows
-        nh, rq, ro = 0, None, None
-        rk, rv = (self._rows(w, x, self.nkv, n, k.dtype) for w, x in (("k", k), ("v", v)))
+        st, n, dt = self._begin(batch), batch.n_rows, k.dtype
+        nh, rq, ro, pos, stride = 0, None, None, None, 0
+        rk, rv = self._rows("k", k, self.nkv, n, dt), self._rows("v", v, self.nkv, n, dt)
         if q is not None:
             nh = q.shape[1]
             if q_out is None:
-                q_out = t.empty((q.shape[0], nh, self.hd), dtype=q.dtype, device=q.device)
-            rq, ro = (C.byref(self._rows(w, x, nh, n, k.dtype)) for w, x in (("q", q), ("q_out", q_out)))
-        stride = 0
+                q_out = _t.empty((q.shape[0], nh, self.hd), dtype=dt, device=self.device)
+            rq, ro = self._rows("q", q, nh, n, dt), self._rows("q_out", q_out, nh, n, dt)
         if rope_pos is not None:
-            if rope_pos.dtype != t.int32 or rope_pos.dim() != 2 or rope_pos.shape[0] < self.axes or rope_pos.shape[1] < n or \
-                    (n > 1 and rope_pos.stride(1) != 1) or rope_pos.device != self.device:
+            if rope_pos.dtype != _t.int32 or rope_pos.dim() != 2 or rope_pos.shape[0] < self.axes or rope_pos.shape[1] < n or \
+                    (n > 1 and rope_pos.stride(1) != 1) or rope_pos.get_device() != self.index:
                 raise ValueError(f"rope_pos is {rope_pos.dtype} {tuple(rope_pos.shape)}, not int32 [{self.axes}, {n}] on {self.device}")
-            stride = rope_pos.stride(0)
-        _check(lib().ornith_hip_paged_append(
-            self.h, C.byref(batch.c), nh, _row_type(k.dtype), C.byref(rk), C.byref(rv), rq, ro, self._vector("q_norm", q_norm),
-            self._vector("k_norm", k_norm), eps, None if rope_pos is None else C.c_void_p(rope_pos.data_ptr()), stride, st),
-            "ornith_hip_paged_append")
+            pos, stride = rope_pos.data_ptr(), rope_pos.stride(0)
+        _check(_lib.ornith_hip_paged_append(self.h, batch.ref, nh, _row_type(dt), rk, rv, rq, ro, self._vector("q_norm", q_norm),
+                                            self._vector("k_norm", k_norm), eps, pos, stride, st), "ornith_hip_paged_append")
         return q_out
 
     def read(self, batch: PagedBatch, dtype, k=None, v=None):
         """(k, v): what is stored at the batch's rows, as values of `dtype`."""
-        t, st = _torch(), self._begin(batch)
-        k, v = (t.empty((batch.n_rows, self.nkv, self.hd), dtype=dtype, device=self.device) if x is None else x for x in (k, v))
-        rk, rv = (self._rows(w, x, self.nkv, batch.n_rows, dtype) for w, x in (("k", k), ("v", v)))
-        _check(lib().ornith_hip_paged_read(self.h, C.byref(batch.c), _row_type(dtype), C.byref(rk), C.byref(rv), st),
-               "ornith_hip_paged_read")
+        st, n = self._begin(batch), batch.n_rows
+        k, v = (_t.empty((n, self.nkv, self.hd), dtype=dtype, device=self.device) if x is None else x for x in (k, v))
+        _check(_lib.ornith_hip_paged_read(self.h, batch.ref, _row_type(dtype), self._rows("k", k, self.nkv, n, dtype),
+                                          self._rows("v", v, self.nkv, n, dtype), st), "ornith_hip_paged_read")
         return k, v
 
     def workspace(self, batch: PagedBatch, nh: int, dtype, n_group: int = 0) -> int:
         """Bytes of workspace that attend (attend_prefix) needs for the batch's sizes and rows of dtype."""
         n = C.c_uint64(0)
-        _check(lib().ornith_hip_paged_workspace(self.h, C.byref(batch.c), nh, _row_type(dtype), n_group, C.byref(n)),
+        _check(_lib.ornith_hip_paged_workspace(self.h, batch.ref, nh, _row_type(dtype), n_group, C.byref(n)),
                "ornith_hip_paged_workspace")
         return n.value
 
@@ -661,31 +662,37 @@ class PagedKV:
         """attend for groups of sequences whose first pages are the same
         (ornith_hip_paged_attend_prefix): int32 prefix_first [n_group + 1] and
         prefix_len [n_group]."""
-        t = _torch()
-        for name, x, n in (("prefix_first", prefix_first, prefix_len.numel() + 1), ("prefix_len", prefix_len, prefix_len.numel())):
-            if x.dtype != t.int32 or x.numel() != n or not x.is_contiguous() or x.device != batch.device:
-                raise ValueError(f"{name}: {n} contiguous int32 on {batch.device}")
+        n = prefix_len.numel()
+        for name, x, n in (("prefix_first", prefix_first, n + 1), ("prefix_len", prefix_len, n)):
+            if x.dtype != _t.int32 or x.numel() != n or not x.is_contiguous() or x.get_device() != self.index:
+                raise ValueError(f"{name}: {n} contiguous int32 on {self.device}")
         return self._attend(batch, q, scale, out, workspace, prefix_first, prefix_len)
 
     def _attend(self, batch, q, scale, out, workspace, first, length):
-        t, st = _torch(), self._begin(batch)
+        st, n, dt = self._begin(batch), batch.n_rows, q.dtype
         nh = q.shape[1] if q.dim() == 3 else 0
-        rq = self._rows("q", q, nh, batch.n_rows, q.dtype)
+        rq = self._rows("q", q, nh, n, dt)
         if out is None:
-            out = t.empty((q.shape[0], nh, self.hd), dtype=q.dtype, device=q.device)
-        ro = self._rows("out", out, nh, batch.n_rows, q.dtype)
+            out = _t.empty((q.shape[0], nh, self.hd), dtype=dt, device=self.device)
+        ro = self._rows("out", out, nh, n, dt)
         n_group = 0 if first is None else length.numel()
         if workspace is None:
-            need = self.workspace(batch, nh, q.dtype, n_group)
-            workspace = t.empty(need, dtype=t.uint8, device=self.device) if need else None
-        size = 0 if workspace is None else workspace.numel() * workspace.element_size()
-        args = (nh, _row_type(q.dtype), C.byref(rq), C.byref(ro), self.hd ** -0.5 if scale is None else scale,
-                C.c_void_p(workspace.data_ptr()) if size else None, size, st)
+            key = (nh, dt, n_group)                      # (a batch's sizes stay, and so do its needs of a pool)
+            needs = batch.needs.setdefault(self, {})
+            need = needs.get(key)
+            if need is None:
+                need = needs[key] = self.workspace(batch, nh, dt, n_group)
+            workspace = _t.empty(need, dtype=_t.uint8, device=self.device) if need else None
+        at, size = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+        if size and (workspace.get_device() != self.index or not workspace.is_contiguous()):
+            raise ValueError(f"workspace: contiguous memory on {self.device}")
+        if scale is None:
+            scale = self.hd ** -0.5
         if first is None:
-            _check(lib().ornith_hip_paged_attend(self.h, C.byref(batch.c), *args), "ornith_hip_paged_attend")
+            _check(_lib.ornith_hip_paged_attend(self.h, batch.ref, nh, _row_type(dt), rq, ro, scale, at, size, st), "ornith_hip_paged_attend")
         else:
-            _check(lib().ornith_hip_paged_attend_prefix(self.h, C.byref(batch.c), n_group, C.c_void_p(first.data_ptr()),
-                                                        C.c_void_p(length.data_ptr()), *args), "ornith_hip_paged_attend_prefix")
+            _check(_lib.ornith_hip_paged_attend_prefix(self.h, batch.ref, n_group, first.data_ptr(), length.data_ptr(), nh, _row_type(dt),
+                                                       rq, ro, scale, at, size, st), "ornith_hip_paged_attend_prefix")
         return out
 
     def check(self) -> None:

@@ -10,6 +10,7 @@
 // O^T += V^T P^T with the probabilities where they are.
 #include "oh_pattn_dev.h"
 #include <algorithm>
+#include <atomic>
 
 namespace {
 
@@ -54,8 +55,9 @@ pattn_many(oh_pattn a, int pieces) {
     // and a batch of one prompt among many single tokens has few idle blocks.
     // Last rows first: they see the most.
     // Blocks go to the eight XCDs in turn, each with an L2 of its own: the pieces of
-    // a head are dealt to those XCDs that hold no other head than they must.
-    const int xcd = blockIdx.x % 8, g8 = gcd8(a.pool.nkv), mine = (int)(blockIdx.x / 8) * (8 / g8) + xcd / g8;
+    // a head are dealt to those XCDs that hold no other head than they must (and
+    // each part's to these from another one on).
+    const int xcd = (blockIdx.x + gcd8(a.pool.nkv) * blockIdx.y) % 8, g8 = gcd8(a.pool.nkv), mine = (int)(blockIdx.x / 8) * (8 / g8) + xcd / g8;
     const int kvh = mine / pieces * g8 + xcd % g8, piece = pieces - 1 - mine % pieces, c = blockIdx.y, G = a.G;
     if (kvh >= a.pool.nkv) return;
     auto first = [&](int i) { return (int64_t)a.b.start[PREFIX ? min(max(a.gfirst[i], 0), a.b.n_seq) : i] * G; };
@@ -442,8 +444,17 @@ hipError_t launch(const oh_pattn *a, int units, int parts, hipStream_t st) {
     const int64_t blocks = 8 * ((pieces * (a->pool.nkv / g8) + 8 / g8 - 1) / (8 / g8));
     if (blocks > kMaxBlocks / 2) return hipErrorInvalidConfiguration;
     const auto k = pattn_many<RT, CT, HD, PREFIX, TURN>;
-    hipError_t e = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) return e;
+    if (lds > 65536) {
+        // (once for each device: a few us a call)
+        static std::atomic<uint64_t> set{0};
+        int dev = 0;
+        hipError_t e = hipGetDevice(&dev);
+        if (e == hipSuccess && !(set >> (dev & 63) & 1)) {
+            e = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+            if (e == hipSuccess) set |= (uint64_t)1 << (dev & 63);
+        }
+        if (e != hipSuccess) return e;
+    }
     hipLaunchKernelGGL(k, dim3((unsigned)blocks, parts), dim3(64 * NW), lds, st, *a, (int)pieces);
     return hipGetLastError();
 }
