@@ -28,13 +28,14 @@ __host__ __device__ inline int gcd8(int n) { return n % 8 == 0 ? 8 : n % 4 == 0 
 template <int RT, int CT, int HD> constexpr bool can_turn() { return RT != OH_PT_F32 && HD < 256 && !(CT == OH_PT_Q8 && HD == 64); }
 template <int RT, int CT, int HD, bool TURN> struct many_cfg {
     static constexpr bool TURNS = TURN;
+    static constexpr int PER_SIMD = can_turn<RT, CT, HD>() || HD == 64 ? 2 : 1;    // waves
     static constexpr int T = HD == 256 ? 32 : 64, NW = TURNS ? 8 : 4, H = T / 32;
     static constexpr int TILE = T * HD * 2;            // keys, or values, of a step in LDS, as 16-bit operands
     static constexpr int LDS = 4 * TILE + 2 * (8 * T + 16);   // two of each; scales and whether there is a page
 };
 
 template <int RT, int CT, int HD, bool PREFIX, bool TURN>
-__global__ void __launch_bounds__((64 * many_cfg<RT, CT, HD, TURN>::NW))
+__global__ void __launch_bounds__((64 * many_cfg<RT, CT, HD, TURN>::NW), (many_cfg<RT, CT, HD, TURN>::PER_SIMD))
 pattn_many(oh_pattn a, int pieces) {
     typedef typename pg_elem<RT>::t row_t;
     typedef pg_ops<RT, CT> ops;
@@ -50,9 +51,10 @@ pattn_many(oh_pattn a, int pieces) {
     int *const lds_ok = (int *)(lds_s + 4 * T);        // [2][2]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hf = lane >> 5;
     // The rows (times heads) are cut at multiples of TR and where units begin; a
-    // block takes one such piece. Unit i's first is piece i + 1 + (cuts up to
-    // it), so the unit of piece x is the last one whose first is not behind it,
-    // and a batch of one prompt among many single tokens has few idle blocks.
+    // block takes one such piece. Unit i's first is piece i + (cuts up to it), so
+    // the unit of piece x is the last one whose first is not behind it, and a
+    // batch of one prompt among many single tokens has few idle blocks. (Idle ones
+    // in turn with busy ones would leave half of the shader engines without work.)
     // Last rows first: they see the most.
     // Blocks go to the eight XCDs in turn, each with an L2 of its own: the pieces of
     // a head are dealt to those XCDs that hold no other head than they must (and
@@ -62,11 +64,11 @@ pattn_many(oh_pattn a, int pieces) {
     if (kvh >= a.pool.nkv) return;
     auto first = [&](int i) { return (int64_t)a.b.start[PREFIX ? min(max(a.gfirst[i], 0), a.b.n_seq) : i] * G; };
     const int n_unit = PREFIX ? a.n_group : a.b.n_seq;
-    const int ui = max(pg_count(n_unit, [&](int i) { return i + 1 + first(i) / TR <= piece; }) - 1, 0);
+    const int ui = max(pg_count(n_unit, [&](int i) { return i + first(i) / TR <= piece; }) - 1, 0);
     pg_unit u;
     if (!pg_unit_at<PREFIX>(a, ui, &u)) return;
     const int F = u.n * G;
-    const int64_t f0 = (int64_t)u.row * G, skip = piece - (ui + 1 + f0 / TR);            // cuts behind the unit's first row
+    const int64_t f0 = (int64_t)u.row * G, skip = piece - (ui + f0 / TR);            // cuts behind the unit's first row
     const int64_t from = skip > 0 ? (f0 / TR + skip) * TR : f0, to = min((f0 / TR + skip + 1) * (int64_t)TR, f0 + F);
     if (skip < 0 || from >= to || (!PREFIX && F <= a.many) || (PREFIX && !u.hi)) return;
     const int parts = pg_parts(u.hi - u.lo, PREFIX ? a.gleast : a.mleast, PREFIX ? a.gparts : a.mparts);
@@ -439,7 +441,7 @@ pattn_many(oh_pattn a, int pieces) {
 template <int RT, int CT, int HD, bool PREFIX, bool TURN>
 hipError_t launch(const oh_pattn *a, int units, int parts, hipStream_t st) {
     constexpr int NW = many_cfg<RT, CT, HD, TURN>::NW, lds = many_cfg<RT, CT, HD, TURN>::LDS;
-    const int64_t pieces = (int64_t)a->b.n_rows * a->G / (32 * NW) + 1 + units;
+    const int64_t pieces = ((int64_t)a->b.n_rows * a->G - 1) / (32 * NW) + units;
     const int g8 = gcd8(a->pool.nkv);                  // heads' residues, each with 8 / g8 XCDs
     const int64_t blocks = 8 * ((pieces * (a->pool.nkv / g8) + 8 / g8 - 1) / (8 / g8));
     if (blocks > kMaxBlocks / 2) return hipErrorInvalidConfiguration;
