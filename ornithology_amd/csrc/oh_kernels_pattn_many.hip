@@ -10,7 +10,6 @@
 // O^T += V^T P^T with the probabilities where they are.
 #include "oh_pattn_dev.h"
 #include <algorithm>
-#include <atomic>
 
 namespace {
 
@@ -22,10 +21,7 @@ constexpr float kBehind = 8.0f;
 // Positions a step, waves a block, and whether the waves take turns: of the two
 // that share a SIMD one has its products while the other has its softmax. That
 // takes eight waves, so two sets of accumulators in a SIMD's registers.
-// the largest power of two up to 8 that divides n
-__host__ __device__ inline int gcd8(int n) { return n % 8 == 0 ? 8 : n % 4 == 0 ? 4 : n % 2 == 0 ? 2 : 1; }
-
-template <int RT, int CT, int HD> constexpr bool can_turn() { return RT != OH_PT_F32 && HD < 256 && !(CT == OH_PT_Q8 && HD == 64); }
+template <int RT, int CT, int HD> constexpr bool can_turn() { return HD < 256 && !(CT == OH_PT_Q8 && HD == 64); }
 template <int RT, int CT, int HD, bool TURN> struct many_cfg {
     static constexpr bool TURNS = TURN;
     static constexpr int PER_SIMD = can_turn<RT, CT, HD>() || HD == 64 ? 2 : 1;    // waves
@@ -44,33 +40,17 @@ pattn_many(oh_pattn a, int pieces) {
     typedef many_cfg<RT, CT, HD, TURN> cfg;
     constexpr bool Q8 = CT == OH_PT_Q8;
     constexpr int NW = cfg::NW, T = cfg::T, H = cfg::H, TILE = cfg::TILE, NT = 64 * NW, TR = 32 * NW;
-    constexpr int NQ = ops::NQ, NP = RT == OH_PT_F32 ? 3 : RT == OH_PT_F16 && Q8 ? 2 : 1, NS = HD / 16, ND = HD / 32;
+    constexpr int NQ = ops::NQ, NP = RT == OH_PT_F16 && Q8 ? 2 : 1, NS = HD / 16, ND = HD / 32;
     extern __shared__ __align__(16) uint8_t lds[];
     uint8_t *const ldk = lds, *const ldv = lds + 2 * TILE;
     float *const lds_s = (float *)(lds + 4 * TILE);    // [2][keys' T, values' T]
     int *const lds_ok = (int *)(lds_s + 4 * T);        // [2][2]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hf = lane >> 5;
-    // The rows (times heads) are cut at multiples of TR and where units begin; a
-    // block takes one such piece. Unit i's first is piece i + (cuts up to it), so
-    // the unit of piece x is the last one whose first is not behind it, and a
-    // batch of one prompt among many single tokens has few idle blocks. (Idle ones
-    // in turn with busy ones would leave half of the shader engines without work.)
-    // Last rows first: they see the most.
-    // Blocks go to the eight XCDs in turn, each with an L2 of its own: the pieces of
-    // a head are dealt to those XCDs that hold no other head than they must (and
-    // each part's to these from another one on).
-    const int xcd = (blockIdx.x + gcd8(a.pool.nkv) * blockIdx.y) % 8, g8 = gcd8(a.pool.nkv), mine = (int)(blockIdx.x / 8) * (8 / g8) + xcd / g8;
-    const int kvh = mine / pieces * g8 + xcd % g8, piece = pieces - 1 - mine % pieces, c = blockIdx.y, G = a.G;
-    if (kvh >= a.pool.nkv) return;
-    auto first = [&](int i) { return (int64_t)a.b.start[PREFIX ? min(max(a.gfirst[i], 0), a.b.n_seq) : i] * G; };
-    const int n_unit = PREFIX ? a.n_group : a.b.n_seq;
-    const int ui = max(pg_count(n_unit, [&](int i) { return i + first(i) / TR <= piece; }) - 1, 0);
+    const int c = blockIdx.y, G = a.G;
     pg_unit u;
-    if (!pg_unit_at<PREFIX>(a, ui, &u)) return;
-    const int F = u.n * G;
-    const int64_t f0 = (int64_t)u.row * G, skip = piece - (ui + f0 / TR);            // cuts behind the unit's first row
-    const int64_t from = skip > 0 ? (f0 / TR + skip) * TR : f0, to = min((f0 / TR + skip + 1) * (int64_t)TR, f0 + F);
-    if (skip < 0 || from >= to || (!PREFIX && F <= a.many) || (PREFIX && !u.hi)) return;
+    int kvh;
+    int64_t from, to;
+    if (!pg_piece<PREFIX, TR>(a, pieces, &u, &kvh, &from, &to)) return;
     const int parts = pg_parts(u.hi - u.lo, PREFIX ? a.gleast : a.mleast, PREFIX ? a.gparts : a.mparts);
     if (c >= parts) return;
     const int64_t pc = PREFIX ? c : a.gparts + c;
@@ -441,22 +421,13 @@ pattn_many(oh_pattn a, int pieces) {
 template <int RT, int CT, int HD, bool PREFIX, bool TURN>
 hipError_t launch(const oh_pattn *a, int units, int parts, hipStream_t st) {
     constexpr int NW = many_cfg<RT, CT, HD, TURN>::NW, lds = many_cfg<RT, CT, HD, TURN>::LDS;
-    const int64_t pieces = ((int64_t)a->b.n_rows * a->G - 1) / (32 * NW) + units;
-    const int g8 = gcd8(a->pool.nkv);                  // heads' residues, each with 8 / g8 XCDs
-    const int64_t blocks = 8 * ((pieces * (a->pool.nkv / g8) + 8 / g8 - 1) / (8 / g8));
+    int64_t blocks;
+    const int64_t pieces = pg_pieces(a, units, 32 * NW, &blocks);
     if (blocks > kMaxBlocks / 2) return hipErrorInvalidConfiguration;
     const auto k = pattn_many<RT, CT, HD, PREFIX, TURN>;
-    if (lds > 65536) {
-        // (once for each device: a few us a call)
-        static std::atomic<uint64_t> set{0};
-        int dev = 0;
-        hipError_t e = hipGetDevice(&dev);
-        if (e == hipSuccess && !(set >> (dev & 63) & 1)) {
-            e = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-            if (e == hipSuccess) set |= (uint64_t)1 << (dev & 63);
-        }
-        if (e != hipSuccess) return e;
-    }
+    static std::atomic<uint64_t> asked{0};
+    const hipError_t e = pg_allow_lds((const void *)k, lds, &asked);
+    if (e != hipSuccess) return e;
     hipLaunchKernelGGL(k, dim3((unsigned)blocks, parts), dim3(64 * NW), lds, st, *a, (int)pieces);
     return hipGetLastError();
 }
@@ -481,5 +452,12 @@ hipError_t go_many(const oh_pattn *a, hipStream_t st) {
 
 } // namespace
 
-extern "C" hipError_t oh_pattn_many_rows(const oh_pattn *a, int *rows) { PG_TYPES(go_rows, a, rows) }
-extern "C" hipError_t oh_launch_pattn_many(const oh_pattn *a, hipStream_t st) { PG_TYPES(go_many, a, st) }
+extern "C" hipError_t oh_pattn_many_rows(const oh_pattn *a, int *rows) {
+    *rows = 128;
+    if (a->type == OH_PT_F32) return hipSuccess;
+    PG_ROWS16(go_rows, a, rows)
+}
+extern "C" hipError_t oh_launch_pattn_many(const oh_pattn *a, hipStream_t st) {
+    if (a->type == OH_PT_F32) return oh_launch_pattn_f32(a, st);
+    PG_ROWS16(go_many, a, st)
+}

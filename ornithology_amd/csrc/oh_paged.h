@@ -89,6 +89,7 @@ hipError_t oh_launch_paged_append(const oh_pappend *a, hipStream_t st);
 hipError_t oh_launch_paged_read(const oh_pappend *a, hipStream_t st);
 hipError_t oh_launch_pattn_few(const oh_pattn *a, hipStream_t st);    // the sequences' (few) and the prefixes' (not gmany)
 hipError_t oh_launch_pattn_many(const oh_pattn *a, hipStream_t st);   // the sequences' (many) and the prefixes' (gmany)
+hipError_t oh_launch_pattn_f32(const oh_pattn *a, hipStream_t st);    // the same for f32 rows
 hipError_t oh_pattn_many_rows(const oh_pattn *a, int *rows);          // of a block, at most, for a's types
 hipError_t oh_launch_pattn_join(const oh_pattn *a, hipStream_t st);
 }

@@ -9,6 +9,8 @@
 #pragma once
 #include "oh_paged_dev.h"
 
+#include <atomic>
+
 // Operand vectors of the matrix instructions. Of the values: fp16 for fp16
 // pools, else bf16, which has f32's range, so that a weight p * scale cannot
 // leave it; codes are exact in either. Of the keys the same, but fp16 over
@@ -181,6 +183,52 @@ OH_DEV void pg_part(const pg_unit &u, int c, int parts, int *t0, int *t1) {
     *t1 = T0 + (int)((int64_t)T * (c + 1) / parts);
 }
 
+// ---- the kernels for many rows ---------------------------------------------------
+// the largest power of two up to 8 that divides n
+__host__ __device__ inline int gcd8(int n) { return n % 8 == 0 ? 8 : n % 4 == 0 ? 4 : n % 2 == 0 ? 2 : 1; }
+
+// The rows (times heads) are cut at multiples of TR and where units begin; a
+// block takes one such piece: rows [from, to) of unit u, for one kv head. Unit i's
+// first is piece i + (cuts up to it), so the unit of piece x is the last one
+// whose first is not behind it, and a batch of one prompt among many single
+// tokens has few idle blocks. (Idle ones in turn with busy ones would leave half
+// of the shader engines without work.) Last rows first: they see the most.
+// Blocks go to the eight XCDs in turn, each with an L2 of its own: the pieces of
+// a head are dealt to those XCDs that hold no other head than they must, and
+// each part's to these from another one on.
+template <bool PREFIX, int TR>
+OH_DEV bool pg_piece(const oh_pattn &a, int pieces, pg_unit *u, int *kvh, int64_t *from, int64_t *to) {
+    const int g8 = gcd8(a.pool.nkv), xcd = (blockIdx.x + g8 * blockIdx.y) % 8, mine = (int)(blockIdx.x / 8) * (8 / g8) + xcd / g8;
+    const int piece = pieces - 1 - mine % pieces, G = a.G, n = PREFIX ? a.n_group : a.b.n_seq;
+    *kvh = mine / pieces * g8 + xcd % g8;
+    if (*kvh >= a.pool.nkv) return false;
+    auto first = [&](int i) { return (int64_t)a.b.start[PREFIX ? min(max(a.gfirst[i], 0), a.b.n_seq) : i] * G; };
+    const int ui = max(pg_count(n, [&](int i) { return i + first(i) / TR <= piece; }) - 1, 0);
+    if (!pg_unit_at<PREFIX>(a, ui, u)) return false;
+    const int64_t F = (int64_t)u->n * G, f0 = (int64_t)u->row * G, skip = piece - (ui + f0 / TR);      // cuts behind the unit's first row
+    *from = skip > 0 ? (f0 / TR + skip) * TR : f0;
+    *to = min((f0 / TR + skip + 1) * (int64_t)TR, f0 + F);
+    return skip >= 0 && *from < *to && (PREFIX ? u->hi > 0 : F > a.many);
+}
+// A kernel's dynamic LDS past 64 KB, asked for once on each device (each time
+// takes a few us); asked: of this kernel, a bit for each device
+inline hipError_t pg_allow_lds(const void *k, int bytes, std::atomic<uint64_t> *asked) {
+    if (bytes <= 65536) return hipSuccess;
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess || (dev < 64 && *asked >> dev & 1)) return e;
+    e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess && dev < 64) *asked |= (uint64_t)1 << dev;
+    return e;
+}
+// pieces, and blocks for them
+inline int64_t pg_pieces(const oh_pattn *a, int units, int rows, int64_t *blocks) {
+    const int64_t pieces = ((int64_t)a->b.n_rows * a->G - 1) / rows + units;
+    const int g8 = gcd8(a->pool.nkv);                  // residues of heads, each with 8 / g8 XCDs
+    *blocks = 8 * ((pieces * (a->pool.nkv / g8) + 8 / g8 - 1) / (8 / g8));
+    return pieces;
+}
+
 // the call f<rows, pool, head dim>(a, st) for a's types
 #define PG_DIMS(f, R, C, a, st)                          \
     switch ((a)->pool.hd) {                              \
@@ -189,9 +237,11 @@ OH_DEV void pg_part(const pg_unit &u, int c, int parts, int *t0, int *t1) {
     case 256: return f<R, C, 256>(a, st);                \
     default: return hipErrorNotSupported;                \
     }
-#define PG_TYPES(f, a, st)                                                          \
+#define PG_ROWS16(f, a, st)                                                         \
     if ((a)->pool.type == OH_PT_BF16) { PG_DIMS(f, OH_PT_BF16, OH_PT_BF16, a, st) } \
     if ((a)->pool.type == OH_PT_F16) { PG_DIMS(f, OH_PT_F16, OH_PT_F16, a, st) }    \
-    if ((a)->type == OH_PT_F32) { PG_DIMS(f, OH_PT_F32, OH_PT_Q8, a, st) }          \
     if ((a)->type == OH_PT_BF16) { PG_DIMS(f, OH_PT_BF16, OH_PT_Q8, a, st) }        \
     PG_DIMS(f, OH_PT_F16, OH_PT_Q8, a, st)
+#define PG_TYPES(f, a, st)                                                          \
+    if ((a)->type == OH_PT_F32) { PG_DIMS(f, OH_PT_F32, OH_PT_Q8, a, st) }          \
+    PG_ROWS16(f, a, st)
