@@ -104,13 +104,16 @@ void plan(const ornith_hip_paged *p, const oh_pbatch &b, int nh, int n_group, oh
     // few rows: 128 positions are a tile for each wave of a block
     if (a->few) a->parts = cut(most, (int64_t)b.n_seq * nkv, 8192, 128, 64, &a->least);
     // Many rows: blocks of 256 rows where units have more than 128 (the wider
-    // block would have idle waves otherwise), and enough of them for the CUs.
+    // block would have idle waves otherwise). Two blocks for each CU, so that
+    // their ends even out; of a prefix, whose blocks are all alike, one for three
+    // of four CUs: the shader engines are not dealt blocks evenly (192 blocks of a
+    // prefix of 8000 positions took 42 us, 252 shorter ones 64).
     int rows = 128;
     (void)oh_pattn_many_rows(a, &rows);
     a->mrows = widest > 128 ? rows : 128;
     a->grows = n_group && all / n_group > 128 ? rows : 128;
-    if (a->many >= 0) a->mparts = cut(most, (all / a->mrows + 1) * nkv, 512, 256, 32, &a->mleast);
-    if (n_group && a->gmany) a->gparts = cut(most, (all / a->grows + n_group) * nkv, a->grows < rows ? 512 : 256, 128, 64, &a->gleast);
+    if (a->many >= 0) a->mparts = cut(most, ((all - 1) / a->mrows + 1) * nkv, 512, 256, 32, &a->mleast);
+    if (n_group && a->gmany) a->gparts = cut(most, ((all - 1) / a->grows + n_group) * nkv, a->grows < rows ? 512 : 192, 128, 64, &a->gleast);
     else if (n_group) a->gparts = cut(most, (int64_t)n_group * nkv, 512, 128, 64, &a->gleast);
     a->sparts = std::max(a->parts, a->mparts);
 }
