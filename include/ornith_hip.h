@@ -277,6 +277,7 @@ typedef struct {
     int32_t n_seq, n_rows;      /* rows that the row buffers hold */
     int32_t max_pages;
     int32_t max_new;            /* no sequence has more rows than this */
+    int32_t max_len;            /* for speed alone: about the longest kv_len (0: what `pages` has room for) */
 } ornith_hip_paged_batch;
 
 /* Rows of heads: element (row, head, d) at p[row * row_stride + head *

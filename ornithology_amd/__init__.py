@@ -61,7 +61,7 @@ class PagedCfg(C.Structure):
 
 class _Batch(C.Structure):
     _fields_ = [("seq_start", C.c_void_p), ("kv_len", C.c_void_p), ("pages", C.c_void_p), ("n_seq", C.c_int32),
-                ("n_rows", C.c_int32), ("max_pages", C.c_int32), ("max_new", C.c_int32)]
+                ("n_rows", C.c_int32), ("max_pages", C.c_int32), ("max_new", C.c_int32), ("max_len", C.c_int32)]
 
 
 class _Rows(C.Structure):
@@ -545,10 +545,10 @@ def _row_type(dtype) -> int:
 class PagedBatch:
     """A ragged batch over a pool's pages (ornith_hip_paged_batch): int32 device
     tensors seq_start [n_seq + 1], kv_len [n_seq] and pages [n_seq, max_pages],
-    whose contents may change between calls; n_rows and max_new are host numbers
-    (default: max_new = n_rows)."""
+    whose contents may change between calls; n_rows, max_new (default: n_rows) and
+    max_len (about the longest kv_len, for speed alone) are host numbers."""
 
-    def __init__(self, seq_start, kv_len, pages, *, n_rows: int, max_new: int | None = None):
+    def __init__(self, seq_start, kv_len, pages, *, n_rows: int, max_new: int | None = None, max_len: int = 0):
         t = _torch()
         n = kv_len.numel()
         for name, x, shape in (("seq_start", seq_start, (n + 1,)), ("kv_len", kv_len, (n,)), ("pages", pages, (n, pages.shape[-1]))):
@@ -559,7 +559,7 @@ class PagedBatch:
         self.seq_start, self.kv_len, self.pages, self.n_rows = seq_start, kv_len, pages, int(n_rows)
         self.device, self.index = kv_len.device, kv_len.get_device()
         self.c = _Batch(seq_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr(), n, self.n_rows, pages.shape[1],
-                        self.n_rows if max_new is None else int(max_new))
+                        self.n_rows if max_new is None else int(max_new), int(max_len))
         self.ref = C.byref(self.c)
         self.needs = weakref.WeakKeyDictionary()   # workspace bytes, by pool and (heads, type, groups)
 

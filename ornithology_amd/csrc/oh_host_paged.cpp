@@ -32,8 +32,9 @@ int type_bytes(uint32_t t) { return t == OH_PT_F32 ? 4 : t == OH_PT_F16 || t == 
 
 int batch_of(const char *who, const ornith_hip_paged *p, const ornith_hip_paged_batch *b, oh_pbatch *out) {
     if (!p || !b) { seterr("%s: null pool or batch", who); return ORNITH_HIP_ERR_FORMAT; }
-    if (b->n_seq < 0 || b->n_rows < 0 || b->max_pages < 0 || b->max_new < 0) {
-        seterr("%s: negative size (n_seq %d, n_rows %d, max_pages %d, max_new %d)", who, b->n_seq, b->n_rows, b->max_pages, b->max_new);
+    if (b->n_seq < 0 || b->n_rows < 0 || b->max_pages < 0 || b->max_new < 0 || b->max_len < 0) {
+        seterr("%s: negative size (n_seq %d, n_rows %d, max_pages %d, max_new %d, max_len %d)", who, b->n_seq, b->n_rows, b->max_pages,
+               b->max_new, b->max_len);
         return ORNITH_HIP_ERR_FORMAT;
     }
     if (b->n_seq && b->n_rows && (!b->seq_start || !b->kv_len || !b->pages)) {
@@ -89,20 +90,20 @@ int cut(int64_t most, int64_t units, int64_t blocks, int64_t least, int limit, i
     *len = (int32_t)std::min<int64_t>(INT32_MAX / 2, std::max(least, (most + n - 1) / n));
     return (int)std::max<int64_t>(1, (most + *len - 1) / *len);
 }
-void plan(const ornith_hip_paged *p, const oh_pbatch &b, int nh, int n_group, oh_pattn *a) {
+void plan(const ornith_hip_paged *p, const oh_pbatch &b, int max_len, int nh, int n_group, oh_pattn *a) {
     const int nkv = p->pool.nkv, G = nh / nkv;
-    const int64_t most = (int64_t)b.max_pages << p->pool.page_sh, widest = (int64_t)b.max_new * G, all = (int64_t)b.n_rows * G;
+    const int64_t table = (int64_t)b.max_pages << p->pool.page_sh, most = max_len > 0 ? std::min<int64_t>(table, max_len) : table, widest = (int64_t)b.max_new * G, all = (int64_t)b.n_rows * G;
     a->G = G;
     a->nh = nh;
     a->n_group = n_group;
     a->few = widest <= kFewRows || (b.n_seq > 1 && b.n_rows < (int64_t)b.n_seq * b.max_new) ? kFewRows : 0;
     a->many = widest <= kFewRows ? -1 : a->few;
     a->gmany = all > kFewRows;
-    a->parts = a->mparts = 1;
-    a->gparts = 0;
+    a->parts = a->mparts = a->gparts = 1;
     a->least = a->mleast = a->gleast = 1;
+    a->few_rows = (int32_t)std::min<int64_t>(b.max_new, std::max(1, kFewRows / G));
     // few rows: 128 positions are a tile for each wave of a block
-    if (a->few) a->parts = cut(most, (int64_t)b.n_seq * nkv, 8192, 128, 64, &a->least);
+    if (a->few) a->parts = cut(most, (int64_t)b.n_seq * nkv, 8192, 128, 256, &a->least);
     // Many rows: blocks of 256 rows where units have more than 128 (the wider
     // block would have idle waves otherwise). Two blocks for each CU, so that
     // their ends even out; of a prefix, whose blocks are all alike, one for three
@@ -115,12 +116,24 @@ void plan(const ornith_hip_paged *p, const oh_pbatch &b, int nh, int n_group, oh
     if (a->many >= 0) a->mparts = cut(most, ((all - 1) / a->mrows + 1) * nkv, 512, 256, 32, &a->mleast);
     if (n_group && a->gmany) a->gparts = cut(most, ((all - 1) / a->grows + n_group) * nkv, a->grows < rows ? 512 : 192, 128, 64, &a->gleast);
     else if (n_group) a->gparts = cut(most, (int64_t)n_group * nkv, 512, 128, 64, &a->gleast);
-    a->sparts = std::max(a->parts, a->mparts);
 }
-uint64_t work_parts(const oh_pattn &a) {
-    return a.sparts == 1 && !a.n_group ? 0 : (uint64_t)a.b.n_rows * a.nh * (a.sparts + a.gparts);
+// The partial results of a call: of the few-row sequences, of those with many
+// rows, of the prefixes; none of a kernel that writes whole rows itself. ws null:
+// the bytes alone.
+uint64_t lay_out(oh_pattn *a, void *ws) {
+    const bool groups = a->n_group > 0;
+    const uint64_t n[3] = {a->few && (groups || a->parts > 1) ? (uint64_t)a->b.n_seq * a->few_rows * a->nh * a->parts : 0,
+                           a->many >= 0 && (groups || a->mparts > 1) ? (uint64_t)a->b.n_rows * a->nh * a->mparts : 0,
+                           groups ? (uint64_t)a->b.n_rows * a->nh * a->gparts : 0};
+    const uint64_t all = n[0] + n[1] + n[2];
+    a->po = (float *)ws;
+    a->mpo = a->po + n[0] * a->pool.hd;
+    a->gpo = a->mpo + n[1] * a->pool.hd;
+    a->pml = (float2 *)(a->po + all * a->pool.hd);
+    a->mpml = a->pml + n[0];
+    a->gpml = a->mpml + n[1];
+    return all * ((uint64_t)a->pool.hd * 4 + 8);
 }
-uint64_t work_bytes(const oh_pattn &a) { return work_parts(a) * ((uint64_t)a.pool.hd * 4 + 8); }
 
 int heads(const char *who, const ornith_hip_paged *p, int nh) {
     if (nh < 1 || nh % p->pool.nkv) {
@@ -152,14 +165,12 @@ int attend(const char *who, const ornith_hip_paged *p, const ornith_hip_paged_ba
     a.scale = fabsf(scale) * 1.44269504088896340736f;
     a.sign = scale < 0.0f ? -1.0f : 1.0f;
     a.gfirst = first; a.glen = shared;
-    plan(p, a.b, nh, n_group, &a);
-    const uint64_t need = work_bytes(a);
+    plan(p, a.b, b->max_len, nh, n_group, &a);
+    const uint64_t need = lay_out(&a, ws);
     if (need > ws_bytes || (need && (!ws || (uintptr_t)ws % 16))) {
         seterr("%s: a 16-byte aligned workspace of %llu bytes is needed, %llu given", who, (unsigned long long)need, (unsigned long long)ws_bytes);
         return ORNITH_HIP_ERR_FORMAT;
     }
-    a.po = (float *)ws;
-    a.pml = (float2 *)(a.po + work_parts(a) * a.pool.hd);
     OnDevice dev(p->ctx->device);
     HCHK(dev.e);
     const hipStream_t st = (hipStream_t)stream;
@@ -337,8 +348,8 @@ extern "C" int ornith_hip_paged_workspace(const ornith_hip_paged *p, const ornit
     CHK(placed("paged_workspace", b));
     a.pool = p->pool;
     a.type = (int)type;
-    plan(p, a.b, nh, n_group, &a);
-    *bytes = work_bytes(a);
+    plan(p, a.b, b->max_len, nh, n_group, &a);
+    *bytes = lay_out(&a, nullptr);
     return ORNITH_HIP_OK;
 }
 

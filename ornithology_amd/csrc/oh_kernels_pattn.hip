@@ -14,7 +14,7 @@ namespace {
 // Work is dealt out in items: (part of the positions, 16 rows, kv head) of a
 // prefix (`groups`: those of this kernel, before the sequences) or sequence. How
 // many a unit has is known on the device only, where the lengths are.
-struct few_item { int rt, kvh, part; bool prefix; };
+struct few_item { int unit, rt, kvh, part; bool prefix; };
 OH_DEV int few_items(const oh_pattn &a, int groups, int x, pg_unit *o) {
     pg_unit &u = *o;
     const bool prefix = x < groups;
@@ -40,6 +40,7 @@ OH_DEV bool few_find(const oh_pattn &a, int groups, int i, few_item *o, pg_unit 
             const int l = __builtin_ctzll(ends);
             const int left = i - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(mine, l));
             o->prefix = x0 + l < groups;
+            o->unit = x0 + l - (o->prefix ? 0 : groups);
             u->row = __builtin_amdgcn_readlane(un.row, l);
             u->n = __builtin_amdgcn_readlane(un.n, l);
             u->lo = __builtin_amdgcn_readlane(un.lo, l);
@@ -77,7 +78,11 @@ pattn_few(oh_pattn a, int groups) {
     const int rt = it.rt, kvh = it.kvh, c = it.part, G = a.G;
     const int F = u.n * G;
     const int parts = pg_parts(u.hi - u.lo, prefix ? a.gleast : a.least, prefix ? a.gparts : a.parts);
-    const int64_t all = a.gparts + a.sparts, pc = prefix ? c : a.gparts + c;
+    // where row `tok`, head h of the item leaves its result
+    auto slot = [&](int tok, int h) {
+        return prefix ? pg_slot_of(a, a.gpo, a.gpml, tok, h, a.gparts, c)
+                      : pg_slot_of(a, a.po, a.pml, (int64_t)it.unit * a.few_rows + tok - u.row, h, a.parts, c);
+    };
     const bool direct = !prefix && parts == 1 && u.lo == 0;
     int t0, t1;
     pg_part(u, c, parts, &t0, &t1);
@@ -276,8 +281,7 @@ pattn_few(oh_pattn a, int groups) {
 #pragma unroll
     for (int w = 0; w < 4; w++) L += sm[w][n] == -INFINITY ? 0.0f : sl[w][n] * pg_exp2(sm[w][n] - M);
     const float mine = m == -INFINITY ? 0.0f : pg_exp2(m - M);
-    const int64_t part = ((int64_t)tok * a.nh + head) * all + pc;
-    if (!direct && wave == 0 && g == 0 && valid) a.pml[part] = make_float2(M, L);
+    if (!direct && wave == 0 && g == 0 && valid) *slot(tok, head).pml = make_float2(M, L);
     // thread x writes row x >> 4, dims 4 (x & 15) .. + 3 of the 64
     const int wr = threadIdx.x >> 4, wd = 4 * (threadIdx.x & 15), wf = rt * 16 + wr;
     const int wtok = u.row + wf / G, whead = kvh * G + wf % G;
@@ -307,7 +311,7 @@ pattn_few(oh_pattn a, int groups) {
             if (direct) {
                 pg_store<4>((row_t *)a.out.p + wtok * a.out.rs + whead * a.out.hs + 64 * q + wd, y);
             } else {
-                *(pg_f4 *)(a.po + (((int64_t)wtok * a.nh + whead) * all + pc) * HD + 64 * q + wd) = (pg_f4){y[0], y[1], y[2], y[3]};
+                *(pg_f4 *)(slot(wtok, whead).po + 64 * q + wd) = (pg_f4){y[0], y[1], y[2], y[3]};
             }
         }
     }
@@ -336,11 +340,14 @@ pattn_join(oh_pattn a) {
     if (parts == 1 && !gparts) return;                 // written already
     const int np = gparts + parts;
     for (int h = blockIdx.y; h < a.nh; h += gridDim.y) {
-    const int64_t at = ((int64_t)r * a.nh + h) * (a.gparts + a.sparts);
     // part c of np: the prefix's, then the sequence's own
-    auto where = [&](int c) { return at + (c < gparts ? c : a.gparts + c - gparts); };
+    auto where = [&](int c) {
+        return c < gparts ? pg_slot_of(a, a.gpo, a.gpml, r, h, a.gparts, c)
+               : few      ? pg_slot_of(a, a.po, a.pml, (int64_t)s * a.few_rows + r - row0, h, a.parts, c - gparts)
+                          : pg_slot_of(a, a.mpo, a.mpml, r, h, a.mparts, c - gparts);
+    };
     float M = -INFINITY;
-    for (int c = lane; c < np; c += 64) M = fmaxf(M, a.pml[where(c)].x);
+    for (int c = lane; c < np; c += 64) M = fmaxf(M, where(c).pml->x);
 #pragma unroll
     for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
     float L = 0.0f;
@@ -349,14 +356,14 @@ pattn_join(oh_pattn a) {
     for (int e = 0; e < E; e++) y[e] = 0.0f;
     for (int c0 = 0; c0 < np; c0 += 64) {
         const int c = c0 + lane;
-        const float2 ml = c < np ? a.pml[where(c)] : make_float2(-INFINITY, 0.0f);
+        const float2 ml = c < np ? *where(c).pml : make_float2(-INFINITY, 0.0f);
         const float w = ml.x == -INFINITY ? 0.0f : pg_exp2(ml.x - M);      // (0: nothing visible in it)
         if (w != 0.0f) L = fmaf(ml.y, w, L);
         const int n = min(64, np - c0);
         for (int i = wave; i < n; i += 16) {           // four requests together; lanes past the last part weigh 0
             fe x[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) x[j] = *(const fe *)(a.po + where(min(c0 + i + 4 * j, np - 1)) * HD + lane * E);
+            for (int j = 0; j < 4; j++) x[j] = *(const fe *)(where(min(c0 + i + 4 * j, np - 1)).po + lane * E);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const float wi = i + 4 * j < n ? __shfl(w, (i + 4 * j) & 63) : 0.0f;

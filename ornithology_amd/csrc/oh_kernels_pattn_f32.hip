@@ -42,7 +42,6 @@ pattn_f32(oh_pattn a, int pieces) {
     if (!pg_piece<PREFIX, TR>(a, pieces, &u, &kvh, &from, &to)) return;
     const int parts = pg_parts(u.hi - u.lo, PREFIX ? a.gleast : a.mleast, PREFIX ? a.gparts : a.mparts);
     if (c >= parts) return;
-    const int64_t pc = PREFIX ? c : a.gparts + c;
     const bool direct = !PREFIX && parts == 1 && u.lo == 0;
     int t0, t1;
     pg_part(u, c, parts, &t0, &t1);
@@ -271,10 +270,10 @@ pattn_f32(oh_pattn a, int pieces) {
 #pragma unroll
         for (int d = 0; d < ND; d++) *(pg_f4 *)(out + 16 * d) = o[d] * inv;
     } else {
-        const int64_t at = ((int64_t)tok * a.nh + head) * (a.gparts + a.sparts) + pc;
-        if (g == 0) a.pml[at] = make_float2(m, l);
+        const pg_slot at = PREFIX ? pg_slot_of(a, a.gpo, a.gpml, tok, head, a.gparts, c) : pg_slot_of(a, a.mpo, a.mpml, tok, head, a.mparts, c);
+        if (g == 0) *at.pml = make_float2(m, l);
 #pragma unroll
-        for (int d = 0; d < ND; d++) *(pg_f4 *)(a.po + at * HD + 16 * d + 4 * g) = o[d];
+        for (int d = 0; d < ND; d++) *(pg_f4 *)(at.po + 16 * d + 4 * g) = o[d];
     }
 }
 

@@ -53,7 +53,6 @@ pattn_many(oh_pattn a, int pieces) {
     if (!pg_piece<PREFIX, TR>(a, pieces, &u, &kvh, &from, &to)) return;
     const int parts = pg_parts(u.hi - u.lo, PREFIX ? a.gleast : a.mleast, PREFIX ? a.gparts : a.mparts);
     if (c >= parts) return;
-    const int64_t pc = PREFIX ? c : a.gparts + c;
     const bool direct = !PREFIX && parts == 1 && u.lo == 0;
     int t0, t1;
     pg_part(u, c, parts, &t0, &t1);
@@ -377,8 +376,9 @@ pattn_many(oh_pattn a, int pieces) {
     }
     if (bad && tid == 0) pg_report(a.pool, OH_PF_PAGE);
     if (!Q8 && __syncthreads_or(odd)) {
-        // dims 32 d + 8 q + 4 hf + i of the lane's row
-        for (int p = max(p0, bmin); p < blim; p++) {
+        // dims 32 d + 8 q + 4 hf + i of the lane's row, over the steps that hid
+        // something (one that did not has added its values: once more changes nothing)
+        for (int p = bad || bmin < p0 ? p0 : p0 + (bmin - p0) / T * T; p < blim; p++) {
             const int page = u.pages[p >> a.pool.page_sh];
             if (p >= lim || !valid || page < 0 || page >= a.pool.n_pages) continue;
             const typename ops::ve *at = (const typename ops::ve *)(pg_block(a.pool, page, kvh) + a.pool.v_off) + pg_v_at(HD, p & page_mask, 4 * hf);
@@ -408,13 +408,13 @@ pattn_many(oh_pattn a, int pieces) {
                 pg_store<4>(to + 32 * d + 8 * q, y);
             }
     } else {
-        const int64_t at = ((int64_t)tok * a.nh + head) * (a.gparts + a.sparts) + pc;
-        if (hf == 0) a.pml[at] = make_float2(m, l);
+        const pg_slot at = PREFIX ? pg_slot_of(a, a.gpo, a.gpml, tok, head, a.gparts, c) : pg_slot_of(a, a.mpo, a.mpml, tok, head, a.mparts, c);
+        if (hf == 0) *at.pml = make_float2(m, l);
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
             for (int q = 0; q < 4; q++)
-                *(pg_f4 *)(a.po + at * HD + 32 * d + 8 * q + 4 * hf) = (pg_f4){o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
+                *(pg_f4 *)(at.po + 32 * d + 8 * q + 4 * hf) = (pg_f4){o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
     }
 }
 

@@ -66,19 +66,22 @@ struct oh_pattn {
     // whole pages within its glen[i] positions
     const int32_t *gfirst, *glen;
     int32_t n_group;
-    // Parts of the key axis, at most (short stretches have fewer): of the
-    // sequences that the kernel for few rows takes, of those that the one for
-    // many takes, of the groups' prefixes. The partial result of row r, head h
-    // and part c is at (r * nh + h) * (gparts + sparts) + c, the prefix's
-    // first; sparts = max(parts, mparts)
-    int32_t parts, mparts, gparts, sparts;
-    int32_t least, mleast, gleast;              // positions of a part, at least
+    // Parts of the key axis, at most (short stretches have fewer), and positions
+    // of one, at least: of the sequences that the kernel for few rows takes, of
+    // those that the one for many takes, of the groups' prefixes
+    int32_t parts, mparts, gparts;
+    int32_t least, mleast, gleast;
     // sequences of up to `few` rows (times heads of a group) go to the one, of
     // more than `many` (-1: none) to the other; prefixes by gmany
     int32_t few, many, gmany;
     int32_t mrows, grows;                       // rows of a block of the latter: 128, or up to oh_pattn_many_rows
-    float *po;                                  // [..][hd], not divided by the sum
-    float2 *pml;                                // [..] running maximum (log2) and sum
+    // Partial results, not divided by the sum, [..][hd], and their running maximum
+    // (log2) and sum: of row j of sequence s, head h and part c at ((s * few_rows +
+    // j) * nh + h) * parts + c; of row r of one with many rows at (r * nh + h) *
+    // mparts + c; of row r over its group's prefix at (r * nh + h) * gparts + c
+    int32_t few_rows;
+    float *po, *mpo, *gpo;
+    float2 *pml, *mpml, *gpml;
 };
 
 // a launch of so many blocks of 256 threads is within the runtime's limits

@@ -2,6 +2,7 @@
 #pragma once
 #include "oh_common.h"
 #include "oh_paged.h"
+#include "oh_paged_layout.h"
 
 typedef __bf16 pg_b8 __attribute__((ext_vector_type(8)));
 typedef _Float16 pg_h8 __attribute__((ext_vector_type(8)));
@@ -16,17 +17,8 @@ template <> struct pg_elem<OH_PT_Q8> { typedef int8_t t; };
 
 OH_DEV void pg_report(const oh_pool &p, int bit) { atomicOr(p.fault, bit); }
 
-// element offsets in a (page, head) block's key and value parts of position
-// `slot` of the page (16-bit and 8-bit pools: units of 8 and 16 elements)
 template <int CT>
-OH_DEV uint32_t pg_k_at(int hd, int slot, int d) {
-    constexpr int U = CT == OH_PT_Q8 ? 16 : 8;
-    return (uint32_t)((slot >> 5) * 32 * hd + ((d / U) * 32 + (slot & 31)) * U + d % U);
-}
-OH_DEV uint32_t pg_v_at(int hd, int slot, int d) {
-    const int s = slot & 31;
-    return (uint32_t)((slot >> 5) * 32 * hd + (((s >> 2) & 3) * hd + d) * 8 + 4 * (s >> 4) + (s & 3));
-}
+OH_DEV uint32_t pg_k_at(int hd, int slot, int d) { return pg_k_place(CT == OH_PT_Q8 ? 16 : 8, hd, slot, d); }
 OH_DEV uint8_t *pg_block(const oh_pool &p, int page, int head) {
     return p.mem + ((size_t)page * p.nkv + head) * p.block;
 }
@@ -45,13 +37,21 @@ OH_DEV int pg_count(int n, P p) {
     }
     return c;
 }
-// The sequence that row r (the same in the whole wave) belongs to, -1 (and
-// reported) if `start` is no ascending list
+// The sequence that row r (the same in the whole wave) belongs to, -1 if none
+// does (and reported, but for rows behind the last sequence). A list that is not
+// ascending leaves the other sequences' rows their own.
 OH_DEV int pg_seq_of_wave(const oh_pool &p, const oh_pbatch &b, int r) {
-    const int s = pg_count(b.n_seq, [&](int i) { return b.start[i + 1] <= r; });
-    if (s >= b.n_seq) return -1;                       // behind the last sequence: nobody's
-    if (r < b.start[s]) { pg_report(p, OH_PF_BATCH); return -1; }
-    return s;
+    for (int i = 0; i < b.n_seq; i += 64) {
+        const int at = i + (int)(threadIdx.x & 63);
+        const uint64_t own = __ballot(at < b.n_seq && b.start[at] <= r && r < b.start[at + 1]);
+        if (!own) continue;
+        const int s = i + __builtin_ctzll(own);
+        if (b.start[s + 1] <= b.n_rows) return s;
+        pg_report(p, OH_PF_BATCH);
+        return -1;
+    }
+    if (r < b.start[b.n_seq]) pg_report(p, OH_PF_BATCH);
+    return -1;
 }
 // the same of a row of the lane's own
 OH_DEV int pg_seq_of(const oh_pool &p, const oh_pbatch &b, int r) {
@@ -66,6 +66,7 @@ OH_DEV int pg_seq_of(const oh_pool &p, const oh_pbatch &b, int r) {
         if (r < b.start[b.n_seq]) pg_report(p, OH_PF_BATCH);
         return -1;
     }
+    if (s1 > b.n_rows) { pg_report(p, OH_PF_BATCH); return -1; }
     return lo;
 }
 

@@ -171,44 +171,34 @@ struct pg_list {
     }
 };
 
-// parts of a stretch of n positions, each of at least `least` and at most `most` of them
-OH_DEV int pg_parts(int n, int least, int most) {
-    const int p = (n + least - 1) / least;
-    return p < 1 ? 1 : p < most ? p : most;
+// where a part's result goes: of row `row` (of a unit: the row itself, or its
+// place among a few rows' slots)
+struct pg_slot { float *po; float2 *pml; };
+OH_DEV pg_slot pg_slot_of(const oh_pattn &a, float *po, float2 *pml, int64_t row, int h, int parts, int c) {
+    const int64_t at = (row * a.nh + h) * parts + c;
+    return {po + at * a.pool.hd, pml + at};
 }
-// the 32-position tiles [t0, t1) of part c of a unit
-OH_DEV void pg_part(const pg_unit &u, int c, int parts, int *t0, int *t1) {
-    const int T0 = u.lo >> 5, T = u.hi > u.lo ? ((u.hi + 31) >> 5) - T0 : 0;
-    *t0 = T0 + (int)((int64_t)T * c / parts);
-    *t1 = T0 + (int)((int64_t)T * (c + 1) / parts);
-}
+
+OH_DEV void pg_part(const pg_unit &u, int c, int parts, int *t0, int *t1) { pg_part(u.lo, u.hi, c, parts, t0, t1); }
 
 // ---- the kernels for many rows ---------------------------------------------------
-// the largest power of two up to 8 that divides n
-__host__ __device__ inline int gcd8(int n) { return n % 8 == 0 ? 8 : n % 4 == 0 ? 4 : n % 2 == 0 ? 2 : 1; }
-
 // The rows (times heads) are cut at multiples of TR and where units begin; a
-// block takes one such piece: rows [from, to) of unit u, for one kv head. Unit i's
-// first is piece i + (cuts up to it), so the unit of piece x is the last one
-// whose first is not behind it, and a batch of one prompt among many single
-// tokens has few idle blocks. (Idle ones in turn with busy ones would leave half
-// of the shader engines without work.) Last rows first: they see the most.
-// Blocks go to the eight XCDs in turn, each with an L2 of its own: the pieces of
-// a head are dealt to those XCDs that hold no other head than they must, and
-// each part's to these from another one on.
+// block takes one such piece: rows [from, to) of unit u, for one kv head. The unit
+// of a piece is the last one whose first piece is not behind it, and a batch of
+// one prompt among many single tokens has few idle blocks. (Idle ones in turn
+// with busy ones would leave half of the shader engines without work.) Last rows
+// first: they see the most. An XCD, with an L2 of its own, has no other heads'
+// pieces than it must.
 template <bool PREFIX, int TR>
 OH_DEV bool pg_piece(const oh_pattn &a, int pieces, pg_unit *u, int *kvh, int64_t *from, int64_t *to) {
-    const int g8 = gcd8(a.pool.nkv), xcd = (blockIdx.x + g8 * blockIdx.y) % 8, mine = (int)(blockIdx.x / 8) * (8 / g8) + xcd / g8;
-    const int piece = pieces - 1 - mine % pieces, G = a.G, n = PREFIX ? a.n_group : a.b.n_seq;
-    *kvh = mine / pieces * g8 + xcd % g8;
+    int64_t piece;
+    pg_block_of(blockIdx.x, blockIdx.y, pieces, a.pool.nkv, kvh, &piece);
     if (*kvh >= a.pool.nkv) return false;
-    auto first = [&](int i) { return (int64_t)a.b.start[PREFIX ? min(max(a.gfirst[i], 0), a.b.n_seq) : i] * G; };
-    const int ui = max(pg_count(n, [&](int i) { return i + first(i) / TR <= piece; }) - 1, 0);
+    auto first = [&](int i) { return (int64_t)a.b.start[PREFIX ? min(max(a.gfirst[i], 0), a.b.n_seq) : i] * a.G; };
+    const int ui = max(pg_count(PREFIX ? a.n_group : a.b.n_seq, [&](int i) { return pg_first_piece(i, first(i), TR) <= piece; }) - 1, 0);
     if (!pg_unit_at<PREFIX>(a, ui, u)) return false;
-    const int64_t F = (int64_t)u->n * G, f0 = (int64_t)u->row * G, skip = piece - (ui + f0 / TR);      // cuts behind the unit's first row
-    *from = skip > 0 ? (f0 / TR + skip) * TR : f0;
-    *to = min((f0 / TR + skip + 1) * (int64_t)TR, f0 + F);
-    return skip >= 0 && *from < *to && (PREFIX ? u->hi > 0 : F > a.many);
+    const int64_t F = (int64_t)u->n * a.G;
+    return pg_piece_rows(piece, ui, (int64_t)u->row * a.G, F, TR, from, to) && (PREFIX ? u->hi > 0 : F > a.many);
 }
 // A kernel's dynamic LDS past 64 KB, asked for once on each device (each time
 // takes a few us); asked: of this kernel, a bit for each device
@@ -223,9 +213,8 @@ inline hipError_t pg_allow_lds(const void *k, int bytes, std::atomic<uint64_t> *
 }
 // pieces, and blocks for them
 inline int64_t pg_pieces(const oh_pattn *a, int units, int rows, int64_t *blocks) {
-    const int64_t pieces = ((int64_t)a->b.n_rows * a->G - 1) / rows + units;
-    const int g8 = gcd8(a->pool.nkv);                  // residues of heads, each with 8 / g8 XCDs
-    *blocks = 8 * ((pieces * (a->pool.nkv / g8) + 8 / g8 - 1) / (8 / g8));
+    const int64_t pieces = pg_piece_count((int64_t)a->b.n_rows * a->G, units, rows);
+    *blocks = pg_blocks(pieces, a->pool.nkv);
     return pieces;
 }
 

@@ -12,6 +12,12 @@ def half_step(dtype):
     return torch.finfo(dtype).eps / 2
 
 
+def half_least(dtype):
+    """How far a rounding to dtype is off at most next to zero: half of its smallest
+    subnormal, whatever the value's own size (fp16: 2^-25)."""
+    return torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+
+
 def rotated(x, w, eps, pos, axis, theta):
     """Rows x [n, heads, hd] normed with weights w (None: not) and rotated:
     pos [axes, n], axis of each frequency."""
@@ -60,7 +66,7 @@ def attention_tolerance(o, spread, reach, dtype, hd, positions, weight_step):
     u = 2.0 ** -24
     score = 4 * math.sqrt(3 * hd) * u * reach + 4 * u * reach
     sums = 4 * math.sqrt(3 * max(1, positions)) * u
-    return half_step(dtype) * o.abs() + spread * (weight_step + 2 * score + sums + 16 * u) + 1e-30
+    return half_step(dtype) * o.abs() + half_least(dtype) + spread * (weight_step + 2 * score + sums + 16 * u) + 1e-30
 
 
 class Made:
