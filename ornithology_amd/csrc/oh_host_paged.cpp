@@ -102,8 +102,11 @@ void plan(const ornith_hip_paged *p, const oh_pbatch &b, int max_len, int nh, in
     a->parts = a->mparts = a->gparts = 1;
     a->least = a->mleast = a->gleast = 1;
     a->few_rows = (int32_t)std::min<int64_t>(b.max_new, std::max(1, kFewRows / G));
-    // few rows: 128 positions are a tile for each wave of a block
-    if (a->few) a->parts = cut(most, (int64_t)b.n_seq * nkv, 8192, 128, 256, &a->least);
+    // Few rows: 128 positions are a tile for each wave of a block; two tiles where
+    // there are many sequences and a block fills a CU (heads of 256), so that short
+    // ones are done in one round of blocks: an item takes about 9 us and 3 for each
+    // further tile
+    if (a->few) a->parts = cut(most, (int64_t)b.n_seq * nkv, 8192, p->pool.hd == 256 && b.n_seq * nkv >= 64 ? 256 : 128, 256, &a->least);
     // Many rows: blocks of 256 rows where units have more than 128 (the wider
     // block would have idle waves otherwise). Two blocks for each CU, so that
     // their ends even out; of a prefix, whose blocks are all alike, one for three

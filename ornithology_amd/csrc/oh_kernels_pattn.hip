@@ -319,18 +319,19 @@ pattn_few(oh_pattn a, int groups) {
     }
 }
 
-// Partial results joined: a block takes one row and some of its heads, each of
-// its waves every fourth part. A lane weighs a part of 64 at a time, so that the loads of
-// the parts' sums wait for no exponential.
-template <int RT, int HD>
+// Partial results joined: a wave takes a head of a row and all of its parts, or,
+// where there are few heads and many parts (SPLIT), a block's waves every fourth
+// part each. A lane
+// weighs a part of 64 at a time, so that the loads of the parts' sums wait for no
+// exponential.
+template <int RT, int HD, bool SPLIT>
 __global__ void __launch_bounds__(256)
 pattn_join(oh_pattn a) {
     typedef typename pg_elem<RT>::t row_t;
-    constexpr int E = HD / 64;
+    constexpr int E = HD / 64, W = SPLIT ? 4 : 1, U = SPLIT ? 4 : 8;       // waves a head, parts requested together
     typedef float fe __attribute__((ext_vector_type(E)));
-    __shared__ float ys[4][HD];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int r = blockIdx.x;
+    __shared__ float ys[SPLIT ? 4 : 1][HD];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = blockIdx.x;
     const int s = pg_seq_of_wave(a.pool, a.b, r);
     int row0, rows, len;
     if (s < 0 || !pg_seq(a, s, &row0, &rows, &len)) return;
@@ -339,51 +340,53 @@ pattn_join(oh_pattn a) {
     const int parts = pg_parts(len - lo, few ? a.least : a.mleast, few ? a.parts : a.mparts), gparts = lo ? pg_parts(lo, a.gleast, a.gparts) : 0;
     if (parts == 1 && !gparts) return;                 // written already
     const int np = gparts + parts;
-    for (int h = blockIdx.y; h < a.nh; h += gridDim.y) {
-    // part c of np: the prefix's, then the sequence's own
-    auto where = [&](int c) {
-        return c < gparts ? pg_slot_of(a, a.gpo, a.gpml, r, h, a.gparts, c)
-               : few      ? pg_slot_of(a, a.po, a.pml, (int64_t)s * a.few_rows + r - row0, h, a.parts, c - gparts)
-                          : pg_slot_of(a, a.mpo, a.mpml, r, h, a.mparts, c - gparts);
-    };
-    float M = -INFINITY;
-    for (int c = lane; c < np; c += 64) M = fmaxf(M, where(c).pml->x);
+    for (int h = SPLIT ? blockIdx.y : 4 * blockIdx.y + wave; h < a.nh; h += (SPLIT ? 1 : 4) * gridDim.y) {
+        // part c of np: the prefix's, then the sequence's own
+        auto where = [&](int c) {
+            return c < gparts ? pg_slot_of(a, a.gpo, a.gpml, r, h, a.gparts, c)
+                   : few      ? pg_slot_of(a, a.po, a.pml, (int64_t)s * a.few_rows + r - row0, h, a.parts, c - gparts)
+                              : pg_slot_of(a, a.mpo, a.mpml, r, h, a.mparts, c - gparts);
+        };
+        float M = -INFINITY;
+        for (int c = lane; c < np; c += 64) M = fmaxf(M, where(c).pml->x);
 #pragma unroll
-    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
-    float L = 0.0f;
-    fe y;
+        for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+        float L = 0.0f;
+        fe y;
 #pragma unroll
-    for (int e = 0; e < E; e++) y[e] = 0.0f;
-    for (int c0 = 0; c0 < np; c0 += 64) {
-        const int c = c0 + lane;
-        const float2 ml = c < np ? *where(c).pml : make_float2(-INFINITY, 0.0f);
-        const float w = ml.x == -INFINITY ? 0.0f : pg_exp2(ml.x - M);      // (0: nothing visible in it)
-        if (w != 0.0f) L = fmaf(ml.y, w, L);
-        const int n = min(64, np - c0);
-        for (int i = wave; i < n; i += 16) {           // four requests together; lanes past the last part weigh 0
-            fe x[4];
+        for (int e = 0; e < E; e++) y[e] = 0.0f;
+        for (int c0 = 0; c0 < np; c0 += 64) {
+            const int c = c0 + lane;
+            const float2 ml = c < np ? *where(c).pml : make_float2(-INFINITY, 0.0f);
+            const float w = ml.x == -INFINITY ? 0.0f : pg_exp2(ml.x - M);  // (0: nothing visible in it)
+            if (w != 0.0f) L = fmaf(ml.y, w, L);
+            const int n = min(64, np - c0);
+            for (int i = SPLIT ? wave : 0; i < n; i += U * W) {            // the last ones again where there are fewer, for nothing
+                fe x[U];
 #pragma unroll
-            for (int j = 0; j < 4; j++) x[j] = *(const fe *)(where(min(c0 + i + 4 * j, np - 1)).po + lane * E);
+                for (int j = 0; j < U; j++) x[j] = *(const fe *)(where(min(c0 + i + W * j, np - 1)).po + lane * E);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float wi = i + 4 * j < n ? __shfl(w, (i + 4 * j) & 63) : 0.0f;
+                for (int j = 0; j < U; j++) {
+                    const float wi = __shfl(w, (i + W * j) & 63);
+                    if (i + W * j >= n) break;
 #pragma unroll
-                for (int e = 0; e < E; e++) y[e] = i + 4 * j < n ? fmaf(x[j][e], wi, y[e]) : y[e];
+                    for (int e = 0; e < E; e++) y[e] = fmaf(x[j][e], wi, y[e]);
+                }
             }
         }
-    }
 #pragma unroll
-    for (int o = 32; o; o >>= 1) L += __shfl_xor(L, o);
+        for (int o = 32; o; o >>= 1) L += __shfl_xor(L, o);
+        const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
+        row_t *to = (row_t *)a.out.p + r * a.out.rs + h * a.out.hs;
+        if (SPLIT) {
+            *(fe *)&ys[wave][lane * E] = y;
+            __syncthreads();
+            for (int d = threadIdx.x; d < HD; d += 256) to[d] = (row_t)(((ys[0][d] + ys[1][d]) + (ys[2][d] + ys[3][d])) * inv);
+            __syncthreads();                           // (ys is the next head's)
+        } else {
 #pragma unroll
-    for (int e = 0; e < E; e++) ys[wave][lane * E + e] = y[e];
-    __syncthreads();
-    const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
-    row_t *to = (row_t *)a.out.p + r * a.out.rs + h * a.out.hs;
-    if ((int)threadIdx.x < HD) {
-        const int d = threadIdx.x;
-        to[d] = (row_t)(((ys[0][d] + ys[1][d]) + (ys[2][d] + ys[3][d])) * inv);
-    }
-    __syncthreads();                                   // (ys is the next head's)
+            for (int e = 0; e < E; e++) to[lane * E + e] = (row_t)(y[e] * inv);
+        }
     }
 }
 
@@ -401,9 +404,11 @@ hipError_t go_few(const oh_pattn *a, hipStream_t st) {
 template <int RT, int CT, int HD>
 hipError_t go_join(const oh_pattn *a, hipStream_t st) {
     // (a prompt's rows have mostly nothing to join: few blocks for them)
-    const int64_t heads = std::min<int64_t>(a->nh, std::max<int64_t>(1, 4096 / a->b.n_rows));
     if (a->b.n_rows > kMaxBlocks) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((pattn_join<RT, HD>), dim3((unsigned)a->b.n_rows, (unsigned)heads), dim3(256), 0, st, *a);
+    const bool split = (int64_t)a->b.n_rows * a->nh <= 256 && std::max(a->parts, a->mparts) + (a->n_group ? a->gparts : 0) > 32;
+    const int64_t blocks = split ? a->nh : (a->nh + 3) / 4, heads = std::min(blocks, std::max<int64_t>(1, (split ? 4096 : 2048) / a->b.n_rows));
+    const auto k = split ? pattn_join<RT, HD, true> : pattn_join<RT, HD, false>;
+    hipLaunchKernelGGL(k, dim3((unsigned)a->b.n_rows, (unsigned)heads), dim3(256), 0, st, *a);
     return hipGetLastError();
 }
 

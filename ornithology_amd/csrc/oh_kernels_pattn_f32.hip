@@ -16,7 +16,7 @@ namespace {
 constexpr float kBehind = 8.0f;                        // (see oh_kernels_pattn_many.hip)
 
 template <int HD> struct f32_cfg {
-    static constexpr int T = HD == 256 ? 32 : 64, NW = 8, H = T / 32;
+    static constexpr int T = 64, NW = 8, H = T / 32;
     static constexpr int TILE = T * HD * 2;            // keys, or values, of a step in LDS, as 16-bit operands
     static constexpr int LDS = 4 * TILE + 2 * (8 * T + 16);   // two of each; scales and whether there is a page
 };
@@ -72,10 +72,10 @@ pattn_f32(oh_pattn a, int pieces) {
     // ---- a step's keys and values: the 32-position tiles' bytes as they are in
     // the pool, 16 a thread at a time; where there is no page (behind the last
     // position, or a bad index) page 0's, which no row looks at
-    constexpr int KB = 32 * HD;                        // bytes of a tile: a load for each thread, or for the first of them
-    static_assert(H * KB <= 16 * NT, "one load a thread");
-    const bool loads = 16 * tid < H * KB;
-    uint4 kr = {}, vr = {};
+    constexpr int KB = 32 * HD, NL = H * KB > 16 * NT ? H * KB / (16 * NT) : 1;      // bytes of a tile; loads per thread
+    static_assert(H * KB == NL * 16 * NT || NL == 1, "whole loads");
+    const bool loads = NL > 1 || 16 * tid < H * KB;    // (a head of 64 keeps half of the threads)
+    uint4 kr[NL] = {}, vr[NL] = {};
     float scl = 0.0f;
     bool ok[H];
     const int page_mask = (1 << a.pool.page_sh) - 1;
@@ -92,12 +92,16 @@ pattn_f32(oh_pattn a, int pieces) {
         *there = page >= 0;
         return pg_block(a.pool, page < 0 ? 0 : page, kvh) + (size_t)((pos & page_mask) >> 5) * KB;
     };
-    auto fetch = [&](pg_list &list, int pos, uint32_t plane, uint4 &r, bool keys = false) {
+    auto fetch = [&](pg_list &list, int pos, uint32_t plane, uint4 (&r)[NL], bool keys = false) {
         const uint8_t *at[H];
         bool there[H];
 #pragma unroll
         for (int h = 0; h < H; h++) at[h] = tile_at(list, pos + 32 * h, &there[h]);
-        if (loads) r = ldg((const uint4 *)((H == 1 || 16 * tid < KB ? at[0] : at[H - 1]) + plane + 16 * tid % KB));
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const int b = 16 * (tid + NT * i);
+            if (loads) r[i] = ldg((const uint4 *)((b < KB ? at[0] : at[H - 1]) + plane + b % KB));
+        }
         if (keys)
 #pragma unroll
             for (int h = 0; h < H; h++) ok[h] = there[h];
@@ -110,12 +114,14 @@ pattn_f32(oh_pattn a, int pieces) {
     // keys: units (8 dims of one position) at (dim / 8 * 32 + position) * 16 of a
     // tile; values: units (8 positions of one dim) at (group * HD + dim) * 16
     auto stage_k = [&](int b) {
-        const int h = 16 * tid / KB, x = tid % (KB / 16), ch = x >> 5, sl = x & 31;           // 16 dims ch of position sl
-        if (loads) {
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const int e = tid + NT * i, h = 16 * e / KB, x = e % (KB / 16), ch = x >> 5, sl = x & 31;        // 16 dims ch of position sl
+            if (!loads) continue;
             kop *to = (kop *)(ldk + b * TILE + h * 64 * HD) + 2 * ch * 32 + sl;
             kop k0, k1;
-            pg_codes(kr.x, kr.y, &k0);
-            pg_codes(kr.z, kr.w, &k1);
+            pg_codes(kr[i].x, kr[i].y, &k0);
+            pg_codes(kr[i].z, kr[i].w, &k1);
             to[0] = k0;
             to[32] = k1;
         }
@@ -125,13 +131,16 @@ pattn_f32(oh_pattn a, int pieces) {
             for (int h = 0; h < H; h++) lds_ok[2 * b + h] = ok[h];
     };
     auto stage_v = [&](int b) {
-        if (!loads) return;
-        vop v0, v1;
-        pg_codes(vr.x, vr.y, &v0);
-        pg_codes(vr.z, vr.w, &v1);
-        vop *to = (vop *)(ldv + b * TILE) + 2 * tid;
-        to[0] = v0;
-        to[1] = v1;
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            if (!loads) continue;
+            vop v0, v1;
+            pg_codes(vr[i].x, vr[i].y, &v0);
+            pg_codes(vr[i].z, vr[i].w, &v1);
+            vop *to = (vop *)(ldv + b * TILE) + 2 * (tid + NT * i);
+            to[0] = v0;
+            to[1] = v1;
+        }
     };
 
     // ---- products: S^T of step t, and O^T of the step before
