@@ -219,26 +219,20 @@ int pool_new(ornith_hip_ctx *ctx, const ornith_hip_paged_cfg *c, ornith_hip_page
     HCHK(dev_malloc(ctx, &p->mem, bytes));
     o.mem = (uint8_t *)p->mem;
     HCHK(hipMemset(p->mem, 0, bytes));
-    // the rotation's (cos, sin): steps of kRopeStep positions, then positions
-    // within one, then the axes; the fault word first
+    // the fault word, the rotation's (cos, sin) of kRopeStep positions each and of
+    // those within one, the axes
     const int steps = half ? (c->max_pos + kRopeStep - 1) / kRopeStep : 0;
-    std::vector<double2> t((size_t)(steps + (half ? kRopeStep : 0)) * half);
-    for (int i = 0; i < half; i++) {
-        const double f = pow((double)c->rope_theta, -2.0 * i / c->rope_dim);
-        for (int k = 0; k < steps; k++) t[(size_t)k * half + i] = {cos((double)k * kRopeStep * f), sin((double)k * kRopeStep * f)};
-        for (int k = 0; k < kRopeStep; k++) t[(size_t)(steps + k) * half + i] = {cos(k * f), sin(k * f)};
-    }
-    const size_t tb = t.size() * sizeof(double2);
-    std::vector<uint8_t> h(256 + tb + half + 1, 0);
-    if (tb) memcpy(h.data() + 256, t.data(), tb);
-    if (half && c->rope_axis) memcpy(h.data() + 256 + tb, c->rope_axis, half);
-    HCHK(dev_malloc(ctx, &p->aux, h.size()));
-    HCHK(hipMemcpy(p->aux, h.data(), h.size(), hipMemcpyHostToDevice));
-    HCHK(hipDeviceSynchronize());
-    o.fault = (int32_t *)p->aux;
-    o.rope_hi = (const double2 *)((uint8_t *)p->aux + 256);
+    const size_t tb = (size_t)(steps + (half ? kRopeStep : 0)) * half * sizeof(double2);
+    HCHK(dev_malloc(ctx, &p->aux, 256 + tb + half + 1));
+    uint8_t *aux = (uint8_t *)p->aux;
+    HCHK(hipMemset(aux, 0, 256 + tb + half + 1));
+    o.fault = (int32_t *)aux;
+    o.rope_hi = (const double2 *)(aux + 256);
     o.rope_lo = o.rope_hi + (size_t)steps * half;
-    o.rope_axis = (uint8_t *)p->aux + 256 + tb;
+    o.rope_axis = aux + 256 + tb;
+    if (half) HCHK(oh_launch_rope_tables((double2 *)(aux + 256), steps, half, c->rope_theta, nullptr));
+    if (half && c->rope_axis) HCHK(hipMemcpy(aux + 256 + tb, c->rope_axis, half, hipMemcpyHostToDevice));
+    HCHK(hipDeviceSynchronize());
     return ORNITH_HIP_OK;
 }
 

@@ -21,6 +21,15 @@ OH_DEV float2 rope_cs(const oh_pool &p, int pos, int i) {
     return make_float2((float)(a.x * b.x - a.y * b.y), (float)(a.y * b.x + a.x * b.y));
 }
 
+// the tables: entries [0, steps) of kRopeStep positions each, then those within one
+__global__ void __launch_bounds__(256) rope_tables(double2 *t, int steps, int half, double theta) {
+    const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int k = (int)(x / half), i = (int)(x % half);
+    if (k >= steps + kRopeStep) return;
+    const double angle = (double)(k < steps ? (int64_t)k * kRopeStep : k - steps) * pow(theta, -(double)i / half);
+    t[x] = make_double2(cos(angle), sin(angle));
+}
+
 // the lanes of one head of one row
 template <int HD> constexpr int head_lanes() { return HD / 8; }
 template <int L, class F>
@@ -85,29 +94,38 @@ OH_DEV void append_qk(const oh_pappend &a, int block, int heads) {
     place at;
     bool ok = place_of(a.pool, a.b, r, &at);
     const int half = a.pool.rope_dim / 2;
-    float2 cs[8];
-    if (half && ok) {
-        bool far = false;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int d = d0 + j, i = d < half ? d : d - half;
-            cs[j] = make_float2(1.0f, 0.0f);
-            if (d < 2 * half) {
-                const int pp = !a.pos ? at.pos : a.pos[(a.axes > 1 ? a.pool.rope_axis[i] : 0) * a.pos_stride + r];
-                if (pp < 0 || pp >= a.pool.max_pos) far = true;
-                else cs[j] = rope_cs(a.pool, pp, i);
-            }
-        }
-        // (one lane's bad position leaves out the row)
-        if (lanes_fold<L>(far ? 1.0f : 0.0f, [](float x, float y) { return fmaxf(x, y); }) > 0.0f) {
-            if (sub == 0) pg_report(a.pool, OH_PF_POSITION);
-            ok = false;
-        }
-    }
     // the other value of a pair: 8 values at a time from another lane where r/2 is a
     // multiple of 8, else one by one
     const bool whole = half % 8 == 0;
-    const int other = d0 < half ? (int)(tid & 63) + half / 8 : (int)(tid & 63) - half / 8;
+    const int other = ((int)(tid & 63) + (d0 < half ? half / 8 : -(half / 8))) & 63;
+    float2 cs[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) cs[j] = make_float2(1.0f, 0.0f);
+    if (half && ok) {
+        int pos[4];
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            pos[x] = x >= a.axes ? 0 : a.pos ? a.pos[x * a.pos_stride + r] : at.pos;
+            if (pos[x] < 0 || pos[x] >= a.pool.max_pos) ok = false;
+        }
+        if (!ok) {
+            if (sub == 0) pg_report(a.pool, OH_PF_POSITION);
+        } else if (d0 < (whole ? half : 2 * half)) {             // (whole: a pair's other lane gets its own from here)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int d = d0 + j, i = d < half ? d : d - half;
+                if (d >= 2 * half) continue;
+                const int x = a.axes > 1 ? a.pool.rope_axis[i] : 0;
+                cs[j] = rope_cs(a.pool, x == 0 ? pos[0] : x == 1 ? pos[1] : x == 2 ? pos[2] : pos[3], i);
+            }
+        }
+    }
+    if (whole)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float x = __shfl(cs[j].x, other), y = __shfl(cs[j].y, other);
+            if (d0 >= half && d0 < 2 * half) cs[j] = make_float2(x, y);
+        }
     for (int hb = h0; hb < h1; hb += U) {
         float y[U][8];
         if (ok) {
@@ -137,7 +155,7 @@ OH_DEV void append_qk(const oh_pappend &a, int block, int heads) {
                 float o[8];
                 if (whole) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++) o[j] = __shfl(y[k][j], other & 63);
+                    for (int j = 0; j < 8; j++) o[j] = __shfl(y[k][j], other);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 8; j++) xs[tid * 8 + j] = y[k][j];
@@ -319,10 +337,10 @@ int span_of(const oh_pappend *a) { return a->b.n_rows >= (int64_t)8 * a->b.n_seq
 template <int RT, int CT, int HD>
 hipError_t append(const oh_pappend *a, hipStream_t st) {
     constexpr int R = 256 / head_lanes<HD>();
-    // as many heads a block as leave 2048 blocks, so that few rows spread over the
+    // as many heads a block as leave 1024 blocks, so that few rows spread over the
     // card and many rows form their sines and cosines once
     const int64_t all = (a->q.p ? a->nh : 0) + a->pool.nkv, chunks = ((int64_t)a->b.n_rows + R - 1) / R;
-    const int64_t heads = std::min(all, std::max<int64_t>(1, chunks * all / 2048));
+    const int64_t heads = std::min(all, std::max<int64_t>(1, chunks * all / 1024));
     const int64_t qk = chunks * ((all + heads - 1) / heads);
     const int span = span_of(a);
     const int64_t v = ((int64_t)a->b.n_rows + span - 1) / span * a->pool.nkv;
@@ -361,3 +379,8 @@ hipError_t types(const oh_pappend *a, bool read, hipStream_t st) {
 
 extern "C" hipError_t oh_launch_paged_append(const oh_pappend *a, hipStream_t st) { return types(a, false, st); }
 extern "C" hipError_t oh_launch_paged_read(const oh_pappend *a, hipStream_t st) { return types(a, true, st); }
+extern "C" hipError_t oh_launch_rope_tables(double2 *t, int steps, int half, double theta, hipStream_t st) {
+    const int64_t n = (int64_t)(steps + kRopeStep) * half;
+    hipLaunchKernelGGL(rope_tables, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, t, steps, half, theta);
+    return hipGetLastError();
+}

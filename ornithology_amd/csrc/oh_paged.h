@@ -88,6 +88,7 @@ struct oh_pattn {
 constexpr int64_t kMaxBlocks = (1 << 24) - 1;
 
 extern "C" {
+hipError_t oh_launch_rope_tables(double2 *t, int steps, int half, double theta, hipStream_t st);
 hipError_t oh_launch_paged_append(const oh_pappend *a, hipStream_t st);
 hipError_t oh_launch_paged_read(const oh_pappend *a, hipStream_t st);
 hipError_t oh_launch_pattn_few(const oh_pattn *a, hipStream_t st);    // the sequences' (few) and the prefixes' (not gmany)
