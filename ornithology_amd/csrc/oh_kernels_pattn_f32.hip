@@ -6,8 +6,10 @@
 // A wave can then hold 16 rows by 16x16x32 products without waiting for LDS,
 // and two waves fit a SIMD's registers at a head dim of 256, where 32 rows a
 // wave left one: its waits for LDS, for the step's loads and for the softmax
-// were all in the open (403 against 332 us for five prompts of 1200 rows at
-// most, 16 heads of 256 over 2).
+// were all in the open (403 us for five prompts of 1200 rows at most, 16 heads
+// of 256 over 2; 332 so, 290 with 64 positions a step instead of 32: 89 GFLOP of
+// scores and sums, 222 in terms). Bound by what the two waves cannot hide from
+// each other: their products fill 40% of the matrix cores' time.
 #include "oh_pattn_dev.h"
 #include <algorithm>
 
@@ -187,13 +189,13 @@ pattn_f32(oh_pattn a, int pieces) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     see[h][u][i] = 16 * u + i < vis;
-                    s[h][u][i] = see[h][u][i] ? s[h][u][i] * kk[i] : -INFINITY;
+                    s[h][u][i] = see[h][u][i] ? s[h][u][i] * (kk[i] * unit) : -INFINITY;
                     mx = fmaxf(mx, s[h][u][i]);
                 }
             }
         }
         mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32)) * unit;
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
         if (__any(mx > m + kBehind)) {
             const float mn = fmaxf(m, mx), alpha = mn == m ? 1.0f : pg_exp2(m - mn);
             m = mn;
@@ -210,7 +212,7 @@ pattn_f32(oh_pattn a, int pieces) {
                 const pg_f4 vv = *(const pg_f4 *)(vs + 32 * h + 16 * u + 4 * g);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float e = pg_exp2(fmaf(s[h][u][i], unit, -ref));
+                    const float e = pg_exp2(s[h][u][i] - ref);
                     l += e;
                     p[4 * u + i] = see[h][u][i] ? e * vv[i] : 0.0f;        // (a hidden scale may be anything)
                 }

@@ -2,12 +2,17 @@
 // group that shares a prefix, brings many rows.
 //
 // A block of NW waves takes 32 NW rows (row, head of one kv head's group) and
-// a part of the positions, 64 at a time: the tile's keys and values go through
-// LDS once for all waves, as matrix operands in the pool's order (codes as
-// bf16), in two buffers, the next tile's loads in flight during this one's
+// a part of the positions, 64 at a time (32 of heads of 256): the tile's keys and
+// values go through LDS once for all waves, as matrix operands in the pool's
+// order (codes as 16-bit values), in two buffers, the next tile's loads in flight during this one's
 // products. A wave holds 32 rows: S^T = K Q^T by 32x32x16 products (lane n =
 // lane & 31 holds row n's scores of half the positions), the softmax, and
 // O^T += V^T P^T with the probabilities where they are.
+//
+// Bound by the matrix cores and LDS: a product of 32 cycles takes 1 KB of LDS for
+// its key or value operand, which is what LDS gives four SIMDs in that time. 8192
+// tokens, 32 heads of 128 over 8, bf16: 0.71 ms, 770 TFLOP/s, where a library
+// product of 8192^3 reaches 1140.
 #include "oh_pattn_dev.h"
 #include <algorithm>
 
