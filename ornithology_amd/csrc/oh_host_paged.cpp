@@ -202,13 +202,22 @@ int pool_new(ornith_hip_ctx *ctx, const ornith_hip_paged_cfg *c, ornith_hip_page
         seterr("paged_new: pool type %u (ORNITH_HIP_KV_Q8, _F16 or _BF16)", c->type);
         return ORNITH_HIP_ERR_UNSUPPORTED;
     }
-    if (c->hd != 64 && c->hd != 128 && c->hd != 256) { seterr("paged_new: head dim %d (64, 128 or 256)", c->hd); return ORNITH_HIP_ERR_UNSUPPORTED; }
+    if (c->hd != 64 && c->hd != 128 && c->hd != 256) {
+        seterr("paged_new: head dim %d (64, 128 or 256)", c->hd);
+        return ORNITH_HIP_ERR_UNSUPPORTED;
+    }
     if (c->page_len != 32 && c->page_len != 64 && c->page_len != 128 && c->page_len != 256) {
         seterr("paged_new: pages of %d positions (32, 64, 128 or 256)", c->page_len);
         return ORNITH_HIP_ERR_UNSUPPORTED;
     }
-    if (c->nkv < 1 || c->nkv > 65535 || c->n_pages < 1) { seterr("paged_new: %d key heads, %d pages", c->nkv, c->n_pages); return ORNITH_HIP_ERR_FORMAT; }
-    if (c->rope_dim < 0 || c->rope_dim > c->hd || c->rope_dim % 2) { seterr("paged_new: rotation of %d of %d dims", c->rope_dim, c->hd); return ORNITH_HIP_ERR_FORMAT; }
+    if (c->nkv < 1 || c->nkv > 65535 || c->n_pages < 1) {
+        seterr("paged_new: %d key heads, %d pages", c->nkv, c->n_pages);
+        return ORNITH_HIP_ERR_FORMAT;
+    }
+    if (c->rope_dim < 0 || c->rope_dim > c->hd || c->rope_dim % 2) {
+        seterr("paged_new: rotation of %d of %d dims", c->rope_dim, c->hd);
+        return ORNITH_HIP_ERR_FORMAT;
+    }
     if (c->rope_dim && (!(c->rope_theta > 0.0f) || !std::isfinite(c->rope_theta) || c->max_pos < 1 || c->max_pos > (1 << 24))) {
         seterr("paged_new: rope_theta %g, max_pos %d (at most 2^24)", (double)c->rope_theta, c->max_pos);
         return ORNITH_HIP_ERR_FORMAT;

@@ -174,6 +174,31 @@ def test_attend(hip_ctx, rows, cache, hd, nh, nkv, page, spec):
     verify(*run_attention(hip_ctx, rows, cache, hd, nh, nkv, page, SPECS[spec]), None, rows)
 
 
+@pytest.mark.parametrize("rows,cache", [("f32", "q8"), ("bf16", "bf16"), ("f16", "q8")])
+@pytest.mark.parametrize("spec", ["one-4097", "padded", "few", "mixed"])
+def test_strided_rows_and_loose_bounds(hip_ctx, rows, cache, spec):
+    m, q, k, v, out = run_attention(hip_ctx, rows, cache, 128, 8, 2, 64, SPECS[spec])
+    held = k.dtype if cache == "q8" else DT[cache]
+    pool = hip_ctx.paged_kv(m.n_pages, 2, 128, page_len=64, type=KV[cache])
+    pool.append(m.whole, k.to(held), v.to(held))
+    stored = pool.read(m.whole, k.dtype)
+    own = m.start[-1]
+    plain = pool.attend(m.batch, q)
+    # one of three row buffers side by side; heads before rows
+    side = torch.full((m.total, 3, 8, 128), 4.0, dtype=q.dtype, device="cuda")
+    side[:, 1] = q
+    heads = torch.full((8, m.total, 128), 4.0, dtype=q.dtype, device="cuda").transpose(0, 1)
+    got = pool.attend(m.batch, side[:, 1], out=heads)
+    assert got is heads and torch.equal(heads[:own], plain[:own]) and (heads[own:] == 4).all()
+    pool.attend(m.batch, heads.copy_(q), out=side[:, 2])
+    assert torch.equal(side[:own, 2], plain[:own]) and (side[:, 0] == 4).all() and (side[own:, 2] == 4).all()
+    # the longest length is a hint, and max_new a bound that may be wide
+    for max_new, max_len in ((max(m.rows), 1), (max(m.rows), 100), (m.total, 0), (m.total + 70, 1 << 20)):
+        batch = oa.PagedBatch(*m.t, n_rows=m.total, max_new=max_new, max_len=max_len)
+        verify(m, q, *stored, pool.attend(batch, q)[:own], None, rows)
+    pool.check()
+
+
 # ---- shared prefixes --------------------------------------------------------------------
 
 GROUPS = {
