@@ -70,9 +70,10 @@ OH_DEV float codes_of(float (&y)[8]) {
     for (int j = 0; j < 8; j++) { am = fmaxf(am, fabsf(y[j])); nan |= y[j] != y[j]; }
     if (nan) am = NAN;
     am = lanes_fold<head_lanes<HD>()>(am, [](float a, float b) { return a != a || b != b ? NAN : fmaxf(a, b); });
-    const float iv = am > 0.0f ? 127.0f / am : 0.0f;
+    // (below 2^-121 127 / max is infinite, and 0 times that no code: such heads are raised first)
+    const float up = am < 0x1p-100f ? 0x1p100f : 1.0f, iv = am > 0.0f ? 127.0f / (am * up) : 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) y[j] = fminf(fmaxf(rintf(y[j] * iv), -127.0f), 127.0f);
+    for (int j = 0; j < 8; j++) y[j] = fminf(fmaxf(rintf(y[j] * up * iv), -127.0f), 127.0f);
     return am / 127.0f;
 }
 OH_DEV uint2 pack_codes(const float (&y)[8]) {

@@ -90,6 +90,23 @@ def test_append_stores_and_rotates(hip_ctx, rows, cache, hd, nh, nkv, page, rope
     pool.check()
 
 
+@pytest.mark.parametrize("size", [2.0 ** -100, 1e-36, 3e-37, 1e-38, 1e-40])
+def test_codes_of_small_heads(hip_ctx, size):
+    g = gen(11)
+    m = Made([40, 1], [40, 70], 32)
+    pool = hip_ctx.paged_kv(m.n_pages, 2, 64, page_len=32, type=oa.KV_Q8)
+    k, v = (torch.randn(m.total, 2, 64, generator=g, device="cuda").clamp(-1, 1) * size for _ in range(2))
+    for x in (k, v):
+        x[:, :, 5] = size                                   # (a head's largest)
+        x[:, :, 7] = 0
+    pool.append(m.batch, k, v)
+    for got, x in zip(pool.read(m.batch, torch.float32), (k, v)):
+        # half a code and the roundings of quotient, scale and product; a subnormal
+        # scale is off by half of 2^-149 in each of up to 127 codes, and its product as much
+        close(got, x.double(), size / 127 * (0.5 + 127 * 5 * 2.0 ** -24) + 128 * 2.0 ** -150)
+        assert (got[:, :, 7] == 0).all()
+
+
 def test_append_in_place_and_without_queries(hip_ctx):
     m = Made([3, 40], [10, 40], 32)
     pool = hip_ctx.paged_kv(m.n_pages, 2, 64, page_len=32, type=oa.KV_BF16, rope_dim=64, rope_theta=1e4)
