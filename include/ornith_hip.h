@@ -281,7 +281,9 @@ typedef struct {
 } ornith_hip_paged_batch;
 
 /* Rows of heads: element (row, head, d) at p[row * row_stride + head *
- * head_stride + d]; pointer and strides (in elements) are multiples of 16 bytes. */
+ * head_stride + d]; pointer and strides (in elements) are multiples of 16 bytes.
+ * Strides of rows that are written are hd at the least where there is more than
+ * one row (head). */
 typedef struct { void *p; int64_t row_stride, head_stride; } ornith_hip_rows;
 
 int  ornith_hip_paged_new(ornith_hip_ctx *ctx, const ornith_hip_paged_cfg *cfg, ornith_hip_paged **out);

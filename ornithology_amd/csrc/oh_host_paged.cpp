@@ -74,6 +74,13 @@ int rows_of(const char *who, const char *what, const ornith_hip_rows *r, uint32_
     return ORNITH_HIP_OK;
 }
 
+// rows that are written: of their own each, so that no two of a launch's stores meet
+int apart(const char *who, const char *what, const oh_prows &r, int64_t n_rows, int64_t heads, int hd) {
+    if ((n_rows < 2 || r.rs >= hd) && (heads < 2 || r.hs >= hd)) return ORNITH_HIP_OK;
+    seterr("%s: rows or heads of %s overlap (strides %lld and %lld, heads of %d)", who, what, (long long)r.rs, (long long)r.hs, hd);
+    return ORNITH_HIP_ERR_FORMAT;
+}
+
 int row_type(const char *who, const ornith_hip_paged *p, uint32_t type) {
     if (type != OH_PT_F32 && type != OH_PT_F16 && type != OH_PT_BF16) {
         seterr("%s: rows of type %u (F32, F16 or BF16)", who, type);
@@ -175,6 +182,8 @@ int attend(const char *who, const ornith_hip_paged *p, const ornith_hip_paged_ba
     if ((int64_t)a.b.n_rows * nh > INT32_MAX || (int64_t)a.b.n_seq * nh > INT32_MAX) CHK(launched(who, hipErrorInvalidConfiguration));
     CHK(rows_of(who, "q", q, type, &a.q));
     CHK(rows_of(who, "out", out, type, &a.out));
+    CHK(apart(who, "out", a.out, b->n_rows, nh, p->pool.hd));
+    if (a.out.p == a.q.p) { seterr("%s: out is q", who); return ORNITH_HIP_ERR_FORMAT; }
     a.pool = p->pool;
     a.type = (int)type;
     a.scale = fabsf(scale) * 1.44269504088896340736f;
@@ -321,6 +330,7 @@ extern "C" int ornith_hip_paged_append(ornith_hip_paged *p, const ornith_hip_pag
         CHK(heads(who, p, nh));
         CHK(rows_of(who, "q", q, type, &a.q));
         CHK(rows_of(who, "q_out", q_out, type, &a.q_out));
+        CHK(apart(who, "q_out", a.q_out, b->n_rows, nh, p->pool.hd));
         a.nh = nh;
     }
     a.pool = p->pool;
@@ -343,6 +353,8 @@ extern "C" int ornith_hip_paged_read(const ornith_hip_paged *p, const ornith_hip
     CHK(placed(who, b));
     CHK(rows_of(who, "k", k, type, &a.k));
     CHK(rows_of(who, "v", v, type, &a.v));
+    CHK(apart(who, "k", a.k, b->n_rows, p->pool.nkv, p->pool.hd));
+    CHK(apart(who, "v", a.v, b->n_rows, p->pool.nkv, p->pool.hd));
     a.pool = p->pool;
     a.type = (int)type;
     OnDevice dev(p->ctx->device);

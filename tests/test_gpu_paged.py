@@ -471,6 +471,25 @@ def test_calls_that_are_refused(hip_ctx):
         pool.attend(m.batch, q)
 
 
+def test_outputs_that_overlap_are_refused(hip_ctx):
+    m, pool, q = filled(hip_ctx, ([1, 2], [10, 90]))
+    k = torch.zeros(m.total, 2, 64, dtype=torch.bfloat16, device="cuda")
+    one, head = torch.zeros(1, 4, 64, dtype=q.dtype, device="cuda").expand(m.total, 4, 64), torch.zeros_like(q)[:, :1].expand_as(q)
+    near = torch.zeros(m.total * 256 + 256, dtype=q.dtype, device="cuda").as_strided(q.shape, (256, 32, 1))
+    for out in (one, head, near):
+        with pytest.raises(oa.HipError, match="overlap"):
+            pool.attend(m.batch, q, out=out)
+        with pytest.raises(oa.HipError, match="overlap"):
+            pool.append(m.batch, k, k, q=q, q_out=out)
+        with pytest.raises(oa.HipError, match="overlap"):
+            pool.read(m.batch, q.dtype, k=torch.empty_like(k), v=out[:, :2])
+    with pytest.raises(oa.HipError, match="out is q"):
+        pool.attend(m.batch, q, out=q)
+    # inputs may: all rows and heads the same
+    assert torch.equal(pool.attend(m.batch, one), pool.attend(m.batch, one.contiguous()))
+    pool.check()
+
+
 # ---- as they are used -----------------------------------------------------------------------
 
 @pytest.mark.parametrize("rows,cache,hd,nh,nkv,page", [("f32", "q8", 256, 16, 2, 64), ("bf16", "bf16", 128, 8, 4, 32)])
